@@ -1,0 +1,423 @@
+// Linear attention with one decay for each head (mathematics: head_decay.cuh), any head sizes up to 256, float or bfloat16.
+//
+//   hd_update_kernel   a block = a segment x a head x 64 x 64 entries of U
+//   hd_pass_kernel     a thread = four (or one) entries of the state of a (sequence, head): walks the segments, leaves S_0 where U was
+//   hd_rows_kernel     a block = a segment x a head: scores, outputs, and with a gate the heads' norm
+//   hd_rates_kernel    the decays of a mixer whose input makes them
+//   hd_step_kernel     one token per sequence: a block = a sequence x a head, the state once through the registers
+//
+// Segments of 64 tokens: the scores of a segment are one tile in shared memory.  Float throughout; bound by multiply-adds on the CUDA cores
+// (the step by the state's way through memory).
+#include "head_decay.cuh"
+#include "memory_common.cuh"
+
+#define HD_SEG 64
+#define HD_PAD 68               // pitch of a tile of 64 columns
+
+// ---- U of a segment ----------------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256) hd_update_kernel(const HeadDecayArgs p) {
+    pdl_sync();
+    __shared__ __align__(16) float ks[32][HD_PAD], vs[32][HD_PAD];
+    __shared__ HdSum c[HD_SEG];
+    const int h = p.h0 + blockIdx.y;
+    const HdSegment s = hd_find(p, blockIdx.x);
+    if (s.b < 0) return;
+    const int tiles = (p.vdim + 63) / 64, r0 = blockIdx.z / tiles * 64, c0 = blockIdx.z % tiles * 64;
+    hd_sums(p, h, s.t0, s.n, c);
+    __syncthreads();
+    const int kv = h / (p.H / p.G);
+    const T* k = static_cast<const T*>(p.k) + (size_t)s.t0 * p.ldk + (size_t)kv * p.dim;
+    const T* v = static_cast<const T*>(p.v) + (size_t)s.t0 * p.ldv + (size_t)kv * p.vdim;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const HdSum last = c[s.n - 1];
+    float acc[4][4] = {};
+    for (int j0 = 0; j0 < s.n; j0 += 32) {
+        for (int e = threadIdx.x; e < 32 * 64; e += 256) {
+            const int j = e >> 6, r = e & 63;
+            const bool in = j0 + j < s.n;
+            ks[j][r] = in && r0 + r < p.dim ? ldf(k + (size_t)(j0 + j) * p.ldk + r0 + r) * expf(hd_minus(last, c[j0 + j])) : 0.f;
+            vs[j][r] = in && c0 + r < p.vdim ? ldf(v + (size_t)(j0 + j) * p.ldv + c0 + r) : 0.f;
+        }
+        __syncthreads();
+#pragma unroll 8
+        for (int j = 0; j < 32; ++j) {
+            const float4 a = *reinterpret_cast<const float4*>(&ks[j][ty * 4]), b = *reinterpret_cast<const float4*>(&vs[j][tx * 4]);
+            const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int l = 0; l < 4; ++l) acc[i][l] += av[i] * bv[l];
+        }
+        __syncthreads();
+    }
+    const size_t at = (size_t)blockIdx.y * p.max_segs + blockIdx.x;
+    float* u = p.work + at * p.dim * p.vdim;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int l = 0; l < 4; ++l) {
+            const int r = r0 + ty * 4 + i, col = c0 + tx * 4 + l;
+            if (r < p.dim && col < p.vdim) u[(size_t)r * p.vdim + col] = acc[i][l];
+        }
+    if (blockIdx.z == 0 && threadIdx.x == 0) p.seg_g[at] = last.hi + last.lo;
+}
+
+// ---- from segment to segment ---------------------------------------------------------------------------------------
+template <int V>
+__global__ void __launch_bounds__(256) hd_pass_kernel(const HeadDecayArgs p) {
+    pdl_sync();
+    const int b = blockIdx.x, h = p.h0 + blockIdx.y, size = p.dim * p.vdim;
+    const int e = (blockIdx.z * 256 + threadIdx.x) * V;
+    int t0, n, slot;
+    if (!hd_sequence(p, b, t0, n, slot) || e >= size) return;
+    float S[V];
+    dm_load<float, V>(p.state + (size_t)slot * p.pitch + (size_t)h * size + e, S);
+    const int segs = (n + p.seg - 1) / p.seg;
+    const size_t first = (size_t)blockIdx.y * p.max_segs + t0 / p.seg + b;
+    float* w = p.work + first * size + e;
+    constexpr int U = 4;
+    for (int i0 = 0; i0 < segs; i0 += U) {
+        float u[U][V], d[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (i0 + i < segs) {
+                dm_load<float, V>(w + (size_t)(i0 + i) * size, u[i]);
+                d[i] = p.seg_g[first + i0 + i];
+            }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (i0 + i < segs) {
+                dm_store<V>(w + (size_t)(i0 + i) * size, S);
+                const float f = expf(d[i]);
+#pragma unroll
+                for (int l = 0; l < V; ++l) S[l] = S[l] * f + u[i][l];
+            }
+    }
+    dm_store<V>(p.new_state + (size_t)slot * p.new_pitch + (size_t)h * size + e, S);
+}
+
+// ---- a segment's outputs --------------------------------------------------------------------------------------------
+// 16 x 16 threads, 4 x 4 results each; columns 64 at a time.  TILES: tiles of 64 columns of vdim.
+template <typename T, int TILES>
+__global__ void __launch_bounds__(256) hd_rows_kernel(const HeadDecayArgs p) {
+    pdl_sync();
+    extern __shared__ __align__(16) float hd_sm[];
+    __shared__ HdSum c[HD_SEG];
+    const int h = p.h0 + blockIdx.y, dim = p.dim, vdim = p.vdim;
+    const HdSegment s = hd_find(p, blockIdx.x);
+    if (s.b < 0) return;
+    hd_sums(p, h, s.t0, s.n, c);
+    float* q_s = hd_sm;                          // [dim][HD_PAD]: q transposed, by token
+    float* p_s = q_s + (size_t)dim * HD_PAD;     // [HD_SEG][HD_PAD]: weights transposed, [key][query]
+    float* x_s = p_s + HD_SEG * HD_PAD;          // [64][HD_PAD]: keys transposed, states, values
+    const int kv = h / (p.H / p.G);
+    const T* q = static_cast<const T*>(p.q) + (size_t)s.t0 * p.ldq + (size_t)h * dim;
+    const T* k = static_cast<const T*>(p.k) + (size_t)s.t0 * p.ldk + (size_t)kv * dim;
+    const T* v = static_cast<const T*>(p.v) + (size_t)s.t0 * p.ldv + (size_t)kv * vdim;
+    const float* S = p.work + ((size_t)blockIdx.y * p.max_segs + blockIdx.x) * dim * vdim;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    for (int e = threadIdx.x; e < HD_SEG * dim; e += 256) {
+        const int i = e / dim, r = e - i * dim;
+        q_s[r * HD_PAD + i] = i < s.n ? ldf(q + (size_t)i * p.ldq + r) : 0.f;
+    }
+    // scores, rows = queries ty * 4 .., columns = keys tx * 4 ..
+    float acc[4][4] = {};
+    auto fma16 = [&](const float* a_row, const float* b_row, float (&r)[4][4]) {
+        const float4 a = *reinterpret_cast<const float4*>(a_row + ty * 4), b = *reinterpret_cast<const float4*>(b_row + tx * 4);
+        const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int l = 0; l < 4; ++l) r[i][l] += av[i] * bv[l];
+    };
+    for (int d0 = 0; d0 < dim; d0 += 64) {
+        const int here = min(64, dim - d0);
+        __syncthreads();
+        for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+            const int j = e >> 6, r = e & 63;
+            if (r < here) x_s[r * HD_PAD + j] = j < s.n ? ldf(k + (size_t)j * p.ldk + d0 + r) : 0.f;
+        }
+        __syncthreads();
+        for (int r = 0; r < here; ++r) fma16(q_s + (size_t)(d0 + r) * HD_PAD, x_s + r * HD_PAD, acc);
+    }
+    // a query sees the keys up to its own; the others' weights are 0 and their values are not multiplied at all
+#pragma unroll
+    for (int l = 0; l < 4; ++l) {
+        const int j = tx * 4 + l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int qi = ty * 4 + i;
+            p_s[j * HD_PAD + qi] = j <= qi && qi < s.n ? acc[i][l] * expf(hd_minus(c[qi], c[j])) : 0.f;
+        }
+    }
+    float from_start[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) from_start[i] = ty * 4 + i < s.n ? expf(c[ty * 4 + i].hi + c[ty * 4 + i].lo) : 0.f;
+    float o[TILES][4][4];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        const int c0 = t * 64;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int l = 0; l < 4; ++l) o[t][i][l] = 0.f;
+        for (int d0 = 0; d0 < dim; d0 += 64) {
+            const int here = min(64, dim - d0);
+            __syncthreads();
+            for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+                const int r = e >> 6, col = e & 63;
+                if (r < here) x_s[r * HD_PAD + col] = c0 + col < vdim ? S[(size_t)(d0 + r) * vdim + c0 + col] : 0.f;
+            }
+            __syncthreads();
+            for (int r = 0; r < here; ++r) fma16(q_s + (size_t)(d0 + r) * HD_PAD, x_s + r * HD_PAD, o[t]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int l = 0; l < 4; ++l) o[t][i][l] *= from_start[i];
+        __syncthreads();
+        for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+            const int j = e >> 6, col = e & 63;
+            x_s[j * HD_PAD + col] = j < s.n && c0 + col < vdim ? ldf(v + (size_t)j * p.ldv + c0 + col) : 0.f;
+        }
+        __syncthreads();
+        const int seen = min(s.n, ty * 4 + 4);
+        for (int j = 0; j < seen; ++j) {
+            if (j <= ty * 4) {
+                fma16(p_s + j * HD_PAD, x_s + j * HD_PAD, o[t]);
+            } else {
+                for (int i = j - ty * 4; i < 4; ++i)
+#pragma unroll
+                    for (int l = 0; l < 4; ++l) {
+                        const float add = p_s[j * HD_PAD + ty * 4 + i] * x_s[j * HD_PAD + tx * 4 + l];
+                        if (i == 1) o[t][1][l] += add;
+                        if (i == 2) o[t][2][l] += add;
+                        if (i == 3) o[t][3][l] += add;
+                    }
+            }
+        }
+    }
+    T* out = static_cast<T*>(p.out) + (size_t)s.t0 * p.ldo + (size_t)h * vdim;
+    const T* gate = static_cast<const T*>(p.gate) + (p.gate ? (size_t)s.t0 * p.ldgate + (size_t)h * vdim : 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int qi = ty * 4 + i;
+        float sq = 0.f;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int l = 0; l < 4; ++l) {
+                o[t][i][l] *= p.scale;
+                sq += o[t][i][l] * o[t][i][l];
+            }
+#pragma unroll
+        for (int m = 8; m > 0; m >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, m);
+        if (qi >= s.n) continue;
+        const float rs = 1.0f / sqrtf(sq / (float)vdim + p.eps);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int l = 0; l < 4; ++l) {
+                const int col = t * 64 + tx * 4 + l;
+                if (col >= vdim) continue;
+                float y = o[t][i][l];
+                if (p.gate) {
+                    const float z = ldf(gate + (size_t)qi * p.ldgate + col);
+                    y = y * rs * p.norm[(size_t)h * vdim + col] * (z / (1.0f + expf(-z)));
+                }
+                stf(out + (size_t)qi * p.ldo + col, y);
+            }
+    }
+}
+
+// ---- one token per sequence ---------------------------------------------------------------------------------------
+// V: columns a thread and access (four where rows and heads are whole 16-byte pieces).
+template <typename T, int V>
+__global__ void __launch_bounds__(256) hd_step_kernel(const HeadDecayArgs p) {
+    constexpr int U = 8;                    // rows asked for together
+    extern __shared__ __align__(16) float hd_sm[];
+    __shared__ float red[33];
+    const int b = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, dim = p.dim, vdim = p.vdim;
+    const int nc = vdim / V, R = 256 / nc;  // columns' threads, groups of rows
+    const int vp = (vdim + 3) / 4 * 4;
+    float* q_s = hd_sm;                     // [dim] each
+    float* k_s = q_s + dim;
+    float* o_s = k_s + dim;                 // [R][vp]
+    pdl_sync();
+    const int slot = p.slots[b];
+    if (slot < 0 || slot >= p.n_slots) return;
+    const int rg = tid / nc, c = (tid - rg * nc) * V;
+    const float* S = p.state + (size_t)slot * p.pitch + (size_t)h * dim * vdim;
+    float* N = p.new_state + (size_t)slot * p.new_pitch + (size_t)h * dim * vdim;
+    float s[U][V];
+    auto fetch = [&](int r0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (r0 + u * R < dim) dm_load<float, V>(S + (size_t)(r0 + u * R) * vdim + c, s[u]);
+    };
+    if (rg < R) fetch(rg);
+    const int kv = h / (p.H / p.G);
+    const T* q = static_cast<const T*>(p.q) + (size_t)b * p.ldq + (size_t)h * dim;
+    const T* k = static_cast<const T*>(p.k) + (size_t)b * p.ldk + (size_t)kv * dim;
+    if (tid < dim) {
+        q_s[tid] = ldf(q + tid) * p.scale;
+        k_s[tid] = ldf(k + tid);
+    }
+    const float decay = expf(hd_log_decay(p.g[(size_t)b * p.g_stride + h]));
+    float v[V] = {};
+    if (rg < R) {
+        const T* vr = static_cast<const T*>(p.v) + (size_t)b * p.ldv + (size_t)kv * vdim + c;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = ldf(vr + e);
+    }
+    float gate = 0.f, nw = 0.f;
+    if (p.gate && tid < vdim) {
+        gate = ldf(static_cast<const T*>(p.gate) + (size_t)b * p.ldgate + (size_t)h * vdim + tid);
+        nw = p.norm[(size_t)h * vdim + tid];
+    }
+    __syncthreads();
+    if (rg < R) {
+        float acc[V] = {};
+        for (int r0 = rg; r0 < dim; r0 += R * U) {
+            if (r0 != rg) fetch(r0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + u * R;
+                if (r >= dim) break;
+                const float qq = q_s[r], kk = k_s[r];
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    s[u][e] = s[u][e] * decay + kk * v[e];
+                    acc[e] += s[u][e] * qq;
+                }
+                dm_store<V>(N + (size_t)r * vdim + c, s[u]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) o_s[rg * vp + c + e] = acc[e];
+    }
+    __syncthreads();
+    float o = 0.f;
+    if (tid < vdim)
+        for (int i = 0; i < R; ++i) o += o_s[i * vp + tid];
+    if (p.gate) {
+        const float rs = 1.0f / sqrtf(block_sum(o * o, red) / (float)vdim + p.eps);
+        o *= rs * nw * (gate / (1.0f + expf(-gate)));
+    }
+    if (tid < vdim) stf(static_cast<T*>(p.out) + (size_t)b * p.ldo + (size_t)h * vdim + tid, o);
+}
+
+// ---- g = -exp(rate) softplus(a + bias) -----------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) hd_rates_kernel(const float* __restrict__ a, const float* __restrict__ rate,
+                                                       const float* __restrict__ bias, float* __restrict__ g, int n, int H) {
+    pdl_sync();
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const float z = a[i] + bias[i % H];
+    g[i] = -expf(rate[i % H]) * (fmaxf(z, 0.f) + log1pf(expf(-fabsf(z))));
+}
+
+// ---- launchers ------------------------------------------------------------------------------------------------------
+static int hd_check(const HeadDecayArgs& p) {
+    if (p.nt < 0 || p.B < 0 || p.H <= 0 || p.G <= 0 || p.H % p.G || p.dim <= 0 || p.vdim <= 0 || p.n_slots < 0 ||
+        p.ldq < (long long)p.H * p.dim || p.ldk < (long long)p.G * p.dim || p.ldv < (long long)p.G * p.vdim ||
+        p.ldo < (long long)p.H * p.vdim || (p.gate && p.ldgate < (long long)p.H * p.vdim) || !p.gate != !p.norm ||
+        p.pitch < (long long)p.H * p.dim * p.vdim || p.new_pitch < (long long)p.H * p.dim * p.vdim ||
+        (p.g_stride != 0 && p.g_stride < p.H))
+        return TB_ERR_ARG;
+    if (p.dim > HD_MAX_DIM || p.vdim > HD_MAX_DIM || p.H > 65535) return TB_ERR_UNSUPPORTED;
+    return 0;
+}
+// Four entries of the states an access: rows, heads and slots are whole 16-byte pieces.
+static bool hd_fours(const HeadDecayArgs& p) {
+    return p.vdim % 4 == 0 && p.pitch % 4 == 0 && p.new_pitch % 4 == 0 && (((uintptr_t)p.state | (uintptr_t)p.new_state) & 15) == 0;
+}
+
+template <typename T, int TILES>
+static void hd_rows_launch(const HeadDecayArgs& p, int heads, cudaStream_t s) {
+    const size_t smem = ((size_t)p.dim + HD_SEG + 64) * HD_PAD * sizeof(float);
+    static PerDevice allowed;
+    tb_allow_smem(allowed, (const void*)hd_rows_kernel<T, TILES>, ((size_t)HD_MAX_DIM + HD_SEG + 64) * HD_PAD * sizeof(float));
+    TB_LAUNCH((hd_rows_kernel<T, TILES>), dim3(p.max_segs, heads), 256, smem, s, p);
+}
+
+// work: floats of scratch, `heads` heads of it (max_segs (dim vdim + 1) each); that many heads are done together.
+template <typename T>
+static int hd_prompt_launch(HeadDecayArgs p, int heads, cudaStream_t s) {
+    const int rc = hd_check(p);
+    if (rc) return rc;
+    if (heads <= 0 || ((uintptr_t)p.work & 15)) return TB_ERR_ARG;
+    if (p.B == 0) return 0;
+    p.seg = HD_SEG;
+    if (p.max_segs < p.nt / p.seg + p.B) return TB_ERR_ARG;
+    p.max_segs = p.nt / p.seg + p.B;
+    const int size = p.dim * p.vdim, tiles = ((p.dim + 63) / 64) * ((p.vdim + 63) / 64);
+    p.seg_g = p.work + (size_t)heads * p.max_segs * size;
+    for (p.h0 = 0; p.h0 < p.H; p.h0 += heads) {
+        const int here = p.H - p.h0 < heads ? p.H - p.h0 : heads;
+        p.heads = here;
+        if (p.nt) TB_LAUNCH((hd_update_kernel<T>), dim3(p.max_segs, here, tiles), 256, 0, s, p);
+        if (hd_fours(p)) TB_LAUNCH((hd_pass_kernel<4>), dim3(p.B, here, (size / 4 + 255) / 256), 256, 0, s, p);
+        else TB_LAUNCH((hd_pass_kernel<1>), dim3(p.B, here, (size + 255) / 256), 256, 0, s, p);
+        if (!p.nt) continue;        // sequences without tokens: their states alone
+        if (p.vdim <= 64) hd_rows_launch<T, 1>(p, here, s);
+        else if (p.vdim <= 128) hd_rows_launch<T, 2>(p, here, s);
+        else hd_rows_launch<T, 4>(p, here, s);
+    }
+    return tb_last_error();
+}
+
+template <typename T>
+static int hd_step_launch(const HeadDecayArgs& p, cudaStream_t s) {
+    const int rc = hd_check(p);
+    if (rc) return rc;
+    if (p.B == 0) return 0;
+    const bool four = hd_fours(p);
+    const int R = 256 / (p.vdim / (four ? 4 : 1)), vp = (p.vdim + 3) / 4 * 4;
+    const size_t smem = (2 * (size_t)p.dim + (size_t)R * vp) * sizeof(float);
+    if (four) TB_LAUNCH((hd_step_kernel<T, 4>), dim3(p.B, p.H), 256, smem, s, p);
+    else TB_LAUNCH((hd_step_kernel<T, 1>), dim3(p.B, p.H), 256, smem, s, p);
+    return tb_last_error();
+}
+
+extern "C" {
+int tb_head_decay_segments(int nt, int B) { return nt / HD_SEG + B; }
+
+int tb_head_decay_rates(const float* a, const float* rate, const float* bias, float* g, int nt, int H, cudaStream_t s) {
+    if (nt < 0 || H <= 0 || (long long)nt * H > 0x7fffffffLL - 256) return TB_ERR_ARG;
+    if (nt == 0) return 0;
+    TB_LAUNCH((hd_rates_kernel), (nt * H + 255) / 256, 256, 0, s, a, rate, bias, g, nt * H, H);
+    return tb_last_error();
+}
+
+#define TB_HEAD_DECAY(SFX, T)                                                                                              \
+    int tb_head_decay_##SFX(const void* q, const void* k, const void* v, const void* gate, long long ldq, long long ldk,   \
+                            long long ldv, long long ldgate, const float* g, int g_stride, const float* norm,              \
+                            const float* state, float* new_state, long long pitch, long long new_pitch, void* out,         \
+                            long long ldo, const int* seq_start, const int* slots, float* work, int max_segs, int heads,   \
+                            int nt, int B, int H, int G, int dim, int vdim, int n_slots, float scale, float eps,           \
+                            cudaStream_t s) {                                                                              \
+        return hd_prompt_launch<T>(HeadDecayArgs{q, k, v, gate, g, norm, state, new_state, out, seq_start, slots, work,    \
+                                                 nullptr, ldq, ldk, ldv, ldgate, ldo, pitch, new_pitch, g_stride, nt, B,   \
+                                                 H, G, dim, vdim, n_slots, max_segs, HD_SEG, 0, H, scale, eps}, heads, s); \
+    }                                                                                                                      \
+    int tb_head_decay_step_##SFX(const void* q, const void* k, const void* v, const void* gate, long long ldq,             \
+                                 long long ldk, long long ldv, long long ldgate, const float* g, int g_stride,             \
+                                 const float* norm, const float* state, float* new_state, long long pitch,                 \
+                                 long long new_pitch, void* out, long long ldo, const int* slots, int B, int H, int G,     \
+                                 int dim, int vdim, int n_slots, float scale, float eps, cudaStream_t s) {                 \
+        return hd_step_launch<T>(HeadDecayArgs{q, k, v, gate, g, norm, state, new_state, out, nullptr, slots, nullptr,     \
+                                               nullptr, ldq, ldk, ldv, ldgate, ldo, pitch, new_pitch, g_stride, B, B, H,   \
+                                               G, dim, vdim, n_slots, 0, HD_SEG, 0, H, scale, eps}, s);                    \
+    }
+TB_HEAD_DECAY(f32, float)
+TB_HEAD_DECAY(bf16, __nv_bfloat16)
+}
+
+#include "tape.h"
+TB_TAPE_REGISTER(tb_head_decay_rates)
+TB_TAPE_REGISTER(tb_head_decay_f32)
+TB_TAPE_REGISTER(tb_head_decay_bf16)
+TB_TAPE_REGISTER(tb_head_decay_step_f32)
+TB_TAPE_REGISTER(tb_head_decay_step_bf16)

@@ -112,6 +112,10 @@ _SIGNATURES: Dict[str, str] = {
     "tb_embed_learned_f32": "pppppiifppp", "tb_embed_learned_bf16": "pppppiifppp",
     "tb_post_add_layernorm_router_f32": "pppppippfipppfipiippppiii",
     "tb_post_add_layernorm_router_bf16": "pppppippfipppfipiippppiii",
+    "tb_head_decay_f32": "ppppllllpipppllplpppiiiiiiiiiff", "tb_head_decay_bf16": "ppppllllpipppllplpppiiiiiiiiiff",
+    "tb_head_decay_step_f32": "ppppllllpipppllplpiiiiiiff", "tb_head_decay_step_bf16": "ppppllllpipppllplpiiiiiiff",
+    "tb_head_decay_rates": "ppppii",
+    "tb_router_groups": "plpppiiiiiiiif",
 }
 class TapeArg(ctypes.Union):
     _fields_ = [("p", ctypes.c_void_p), ("i", ctypes.c_int), ("f", ctypes.c_float), ("l", ctypes.c_longlong),
@@ -132,7 +136,8 @@ class TapeMap(ctypes.Structure):
     _fields_ = [("base", ctypes.c_ulonglong), ("size", ctypes.c_ulonglong), ("delta", ctypes.c_longlong)]
 
 
-_NO_STREAM = {"tb_decay_scan_rect_record_size": "ii", "tb_split_delta_record_size": "i",
+_NO_STREAM = {"tb_head_decay_segments": "ii",
+              "tb_decay_scan_rect_record_size": "ii", "tb_split_delta_record_size": "i",
               "tb_decay_state_size": "iii", "tb_decay_record_size": "i",
               "tb_attention_window_mma_tile_tokens": "ii", "tb_delta_state_size": "iiiii", "tb_delta_record_size": "i", "tb_delta_scan_lanes": "i", "tb_delta_chunk_record_size": "iii", "tb_delta_chunk_tokens": "", "tb_delta_value_pitch": "i", "tb_mlstm_state_size": "ii", "tb_mlstm_parallel_size": "iiii", "tb_mlstm_parallel_gates": "", "tb_mlstm_parallel_tokens": "", "tb_latent_attention_tile_tokens": "i", "tb_latent_tc_tile_tokens": "iii", "tb_attention_tile_tokens": "ii", "tb_gemm_tc_takes_pairs": "iiiiiii", "tb_gemm_tc_status": "", "tb_attention_prefill_tile_tokens": "",
               "tb_attention_tc_tile_tokens": ""}
@@ -359,6 +364,16 @@ def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def check_device(*tensors) -> None:
+    """ValueError unless all tensors (None aside) lie on the CUDA device that is current: a kernel is launched there."""
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {device} and on {t.device} in one call")
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise ValueError(f"the tensors lie on {device}, which is not the current CUDA device")
+
+
 def suffix(dtype: torch.dtype) -> str:
     if dtype == torch.float32:
         return "f32"
@@ -486,6 +501,11 @@ def gated_linear_record_size(dim: int, vdim: int) -> int:
 def split_delta_record_size(dim: int) -> int:
     """Floats of the record that the split delta rule's first kernel leaves the scan per (token, head)."""
     return library().tb_split_delta_record_size(dim)
+
+
+def head_decay_segments(tokens: int, sequences: int) -> int:
+    """Segments that a step's tokens are cut into at most, for the linear attention with one decay a head."""
+    return library().tb_head_decay_segments(tokens, sequences)
 
 
 def attention_window_mma_tile_tokens(nh: int, nkvh: int) -> int:

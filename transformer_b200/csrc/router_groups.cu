@@ -1,0 +1,301 @@
+// The choice of experts within groups, from router logits x [nt, E] in float:
+//
+//   s = softmax(x) or sigmoid(x);   c = s + bias (the bias steers the choice alone)
+//   a group's worth = the sum of its group_top (1 or 2) largest c;  the groups_use worthiest groups stay
+//   the k largest c of those are chosen, in descending order;  w = s of the chosen, / their sum with `renorm`, times `scale`
+//
+// Equal c, or groups of equal worth, go to the lower index.  An expert with logit -inf has s = 0 (in a row of nothing else too); NaN ranks
+// below -inf, so the k indices of a row always differ; chosen scores that are all 0 stay 0 when they are renormalized.
+//
+// A warp per token, a lane the PER neighbouring experts from lane * PER on: the lowest lane among equals has the lowest index, so
+// a choice is one redux over order-preserving keys, a ballot and a shuffle.  Without a bias c and x have the same order, and the
+// logits themselves are compared.  With one, or where sums of scores decide, values closer than what float rounding can turn round
+// are decided again in 64 bits (float: expf 2 ulp, two more roundings, the sum's): a row in some hundreds.
+// Bound by instructions: 8,191 tokens of 256 experts are 8.4 MB.
+#include "common.cuh"
+
+#define RG_MAX_E 1024
+#define RG_MAX_K 31
+#define RG_MAX_GROUPS 32
+#define RG_WARPS 8
+
+struct RouterGroupArgs {
+    const float* logits;            // [nt] rows of E, ld apart
+    const float* bias;              // [E] or null
+    int* idx;                       // [nt, k]
+    float* w;
+    long long ld;
+    int nt, E, k, groups, groups_use, group_top, softmax, renorm;
+    float scale;
+};
+
+// larger value <=> larger key; NaN 1; 0 is left for what cannot be chosen (any more)
+__device__ __forceinline__ unsigned rg_key(float c) {
+    const unsigned b = __float_as_uint(c + 0.0f);
+    return c != c ? 1u : b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float rg_value(unsigned key) {
+    return key == 1u ? __int_as_float(0x7fc00000) : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+// c of expert e in 64 bits; NaN as below every number.
+__device__ __forceinline__ double rg_rank64(const RouterGroupArgs& p, float x, int e, float mx, double inv) {
+    const double s = p.softmax ? exp((double)x - (double)mx) * inv : 1.0 / (1.0 + exp(-(double)x));
+    return s + (p.bias ? (double)p.bias[e] : 0.0);
+}
+
+// The choice in 64 bits, by plain steps: called for the few rows where float cannot tell.  Returns this lane's choice (lane < k).
+template <int PER>
+__device__ __noinline__ int rg_choose64(const RouterGroupArgs& p, const float* row, float mx, int lane) {
+    const double lowest = -INFINITY;
+    double c[PER], sum = 0.0;
+    bool open[PER];                 // may be chosen
+    for (int i = 0; i < PER; ++i) {
+        const int e = lane * PER + i;
+        open[i] = e < p.E;
+        if (open[i] && p.softmax) sum += exp((double)row[e] - (double)mx);
+    }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const double inv = sum > 0.0 ? 1.0 / sum : sum == 0.0 ? 0.0 : sum;
+    for (int i = 0; i < PER; ++i) c[i] = open[i] ? rg_rank64(p, row[lane * PER + i], lane * PER + i, mx, inv) : lowest;
+    if (p.groups > 1) {
+        const int size = p.E / p.groups;
+        double worth = lowest;      // of group `lane`
+        for (int g = 0; g < p.groups; ++g) {
+            double a = lowest, b = lowest;      // the two largest
+            for (int i = 0; i < PER; ++i)
+                if (open[i] && (lane * PER + i) / size == g) {
+                    if (c[i] > a) { b = a; a = c[i]; }
+                    else if (c[i] > b) b = c[i];
+                }
+            for (int o = 16; o > 0; o >>= 1) {
+                const double oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+                b = oa > a ? fmax(a, ob) : fmax(b, oa);
+                a = fmax(a, oa);
+            }
+            if (lane == g) worth = p.group_top == 2 && size > 1 ? a + b : a;
+        }
+        int place = 0;
+        for (int g = 0; g < p.groups; ++g) {
+            const double other = __shfl_sync(0xffffffffu, worth, g);
+            place += other > worth || (other == worth && g < lane);
+        }
+        const unsigned kept = __ballot_sync(0xffffffffu, lane < p.groups && place < p.groups_use);
+        for (int i = 0; i < PER; ++i) open[i] = open[i] && (kept >> ((lane * PER + i) / size) & 1u);
+    }
+    int mine = 0;
+    for (int j = 0; j < p.k; ++j) {
+        double best = lowest;
+        int at = 0x7fffffff;
+        for (int i = 0; i < PER; ++i) {
+            const double v = c[i] != c[i] ? lowest : c[i];
+            if (open[i] && (at == 0x7fffffff || v > best)) {
+                best = v;
+                at = lane * PER + i;
+            }
+        }
+        for (int o = 16; o > 0; o >>= 1) {
+            const double ov = __shfl_xor_sync(0xffffffffu, best, o);
+            const int oi = __shfl_xor_sync(0xffffffffu, at, o);
+            if (oi != 0x7fffffff && (at == 0x7fffffff || ov > best || (ov == best && oi < at))) {
+                best = ov;
+                at = oi;
+            }
+        }
+        for (int i = 0; i < PER; ++i)
+            if (lane * PER + i == at) open[i] = false;
+        if (lane == j) mine = at;
+    }
+    return mine;
+}
+
+template <int PER>
+__global__ void __launch_bounds__(RG_WARPS * 32) router_groups_kernel(const RouterGroupArgs p) {
+    extern __shared__ float rg_sm[];        // [RG_WARPS][E + E / 32 + 1] where groups' worths are found
+    pdl_sync();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long t = (long long)blockIdx.x * RG_WARPS + warp;
+    if (t >= p.nt) return;
+    const float* row = p.logits + t * p.ld;
+    const int E = p.E, e0 = lane * PER;
+    float x[PER];
+    if (PER >= 4 && (((uintptr_t)row & 15) == 0)) {
+#pragma unroll
+        for (int i = 0; i < PER; i += 4) {
+            if (e0 + i + 4 <= E) {
+                const float4 f = *reinterpret_cast<const float4*>(row + e0 + i);
+                x[i] = f.x;
+                if (PER >= 4) {
+                    x[(i + 1) % PER] = f.y;
+                    x[(i + 2) % PER] = f.z;
+                    x[(i + 3) % PER] = f.w;
+                }
+            } else {
+#pragma unroll
+                for (int l = 0; l < 4; ++l) x[(i + l) % PER] = e0 + i + l < E ? row[e0 + i + l] : -INFINITY;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x[i] = e0 + i < E ? row[e0 + i] : -INFINITY;
+    }
+    // scores, as far as they are asked for
+    const bool sums = p.groups > 1 && p.group_top == 2;     // sums of scores decide
+    const bool by_logit = !p.bias;
+    float mx = 0.f, inv = 1.f;
+    if (p.softmax && (p.bias || sums || !p.renorm)) {
+        mx = x[0];
+#pragma unroll
+        for (int i = 1; i < PER; ++i) mx = fmaxf(mx, x[i]);
+        mx = warp_max(mx);
+        if (mx == -INFINITY) mx = 0.f;      // a row of masked experts: scores of 0
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) sum += expf(x[i] - mx);
+        sum = warp_sum(sum);
+        inv = sum == 0.f ? 0.f : 1.0f / sum;
+    }
+    auto score = [&](float v) { return p.softmax ? expf(v - mx) * inv : 1.0f / (1.0f + expf(-v)); };
+    unsigned key[PER];
+    float c[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        c[i] = by_logit && !sums ? x[i] : score(x[i]);
+        if (p.bias && e0 + i < E) c[i] += p.bias[e0 + i];
+        key[i] = e0 + i < E ? rg_key(by_logit ? x[i] : c[i]) : 0u;
+    }
+    // what float may have turned round: scores up to `top`, each off by up to 4 (sigmoid) or 24 (softmax, its sum included)
+    // half steps of it, and the roundings of the sums that were compared
+    const float loose = (p.softmax ? 24.f * inv : 4.f) * 1.2e-7f;
+    bool again = false;
+    if (p.groups > 1) {
+        // 32 / groups lanes (a power of two) find a group's worth
+        float* cs = rg_sm + (size_t)warp * (E + E / 32 + 1);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (e0 + i < E) cs[e0 + i + ((e0 + i) >> 5)] = c[i] != c[i] ? -INFINITY : c[i];
+        __syncwarp();
+        const int size = E / p.groups;
+        int L = 1;
+        while (2 * L * p.groups <= 32) L *= 2;
+        const int g = lane / L, part = lane - g * L;
+        float a = -INFINITY, b = -INFINITY;
+        if (g < p.groups)
+            for (int i = part; i < size; i += L) {
+                const int e = g * size + i;
+                const float v = cs[e + (e >> 5)];
+                b = fmaxf(b, fminf(a, v));
+                a = fmaxf(a, v);
+            }
+        for (int o = L >> 1; o > 0; o >>= 1) {
+            const float oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+            b = fmaxf(fminf(a, oa), fmaxf(b, ob));
+            a = fmaxf(a, oa);
+        }
+        const float worth = p.group_top == 2 && size > 1 ? a + b : a;
+        int place = 0;
+        for (int j = 0; j < p.groups; ++j) {
+            const float other = __shfl_sync(0xffffffffu, worth, j * L);
+            place += other > worth || (other == worth && j < g);
+        }
+        const bool in = g < p.groups && place < p.groups_use;
+        if (!(by_logit && !sums) && p.groups_use < p.groups) {
+            float least = in ? worth : INFINITY, most = g < p.groups && !in ? worth : -INFINITY;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            }
+            again = least - most <= 4.f * loose + 2.5e-7f * (fabsf(least) + fabsf(most));
+        }
+        const unsigned kept = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (e0 + i < E && !(kept >> ((e0 + i) / size * L) & 1u)) key[i] = 0u;
+    }
+    // the k largest, and the one that would come next
+    unsigned most = key[0], my_key = 0u;
+#pragma unroll
+    for (int i = 1; i < PER; ++i) most = max(most, key[i]);
+    int mine = 0;
+    for (int j = 0; j <= p.k; ++j) {
+        const unsigned best = __reduce_max_sync(0xffffffffu, most);
+        const int from = __ffs(__ballot_sync(0xffffffffu, most == best)) - 1;
+        int at = 0;
+        if (lane == from) {
+            bool found = false;
+            most = 0u;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                if (!found && key[i] == best) {
+                    found = true;
+                    at = e0 + i;
+                    key[i] = 0u;
+                }
+                most = max(most, key[i]);
+            }
+        }
+        at = __shfl_sync(0xffffffffu, at, from);
+        if (lane == j) {
+            my_key = best;
+            mine = at;
+        }
+    }
+    float mine_x = lane <= p.k && my_key ? row[mine] : 0.f;
+    if (!by_logit) {
+        const float v = rg_value(my_key), nv = __shfl_down_sync(0xffffffffu, v, 1), nx = __shfl_down_sync(0xffffffffu, mine_x, 1);
+        const unsigned nk = __shfl_down_sync(0xffffffffu, my_key, 1);
+        const float mb = lane <= p.k && my_key ? p.bias[mine] : 0.f, nb = __shfl_down_sync(0xffffffffu, mb, 1);
+        const bool close = lane < p.k && my_key && nk && v - nv <= 2.f * loose + 1.3e-7f * (fabsf(v) + fabsf(nv)) &&
+                           !(mine_x == nx && mb == nb);
+        again = again || close;
+    }
+    if (__any_sync(0xffffffffu, again)) {
+        mine = rg_choose64<PER>(p, row, mx, lane);
+        if (lane < p.k) mine_x = row[mine];
+    }
+    // weights
+    float s = 0.f;
+    if (p.renorm) {
+        // against the largest chosen logit, so that small scores keep their ratios
+        float m = lane < p.k ? mine_x : -INFINITY;
+        m = warp_max(m);
+        if (!p.softmax) m = fminf(m, 0.f);
+        if (m == -INFINITY) m = 0.f;
+        if (lane < p.k) s = p.softmax ? expf(mine_x - m) : m < 0.f ? expf(mine_x - m) / (1.0f + expf(mine_x)) : 1.0f / (1.0f + expf(-mine_x));
+        const float sum = warp_sum(s);
+        if (sum != 0.f) s /= sum;
+    } else if (lane < p.k) {
+        s = score(mine_x);
+    }
+    if (lane < p.k) {
+        p.idx[t * p.k + lane] = mine;
+        p.w[t * p.k + lane] = s * p.scale;
+    }
+}
+
+template <int PER>
+static void router_groups_launch(const RouterGroupArgs& p, cudaStream_t s) {
+    const size_t smem = p.groups > 1 ? (size_t)RG_WARPS * (p.E + p.E / 32 + 1) * sizeof(float) : 0;
+    TB_LAUNCH((router_groups_kernel<PER>), (p.nt + RG_WARPS - 1) / RG_WARPS, RG_WARPS * 32, smem, s, p);
+}
+
+extern "C" int tb_router_groups(const float* logits, long long ld, const float* bias, int* idx, float* w, int nt, int E, int k,
+                                int groups, int groups_use, int group_top, int softmax, int renorm, float scale, cudaStream_t s) {
+    if (nt < 0 || E <= 0 || k <= 0 || groups <= 0 || E % groups || groups_use <= 0 || groups_use > groups || ld < E ||
+        k > E / groups * groups_use || group_top < 1 || group_top > 2)
+        return TB_ERR_ARG;
+    if (E > RG_MAX_E || k > RG_MAX_K || groups > RG_MAX_GROUPS) return TB_ERR_UNSUPPORTED;
+    if (nt == 0) return 0;
+    const RouterGroupArgs p{logits, bias, idx, w, ld, nt, E, k, groups, groups_use, group_top, softmax, renorm, scale};
+    if (E <= 32) router_groups_launch<1>(p, s);
+    else if (E <= 64) router_groups_launch<2>(p, s);
+    else if (E <= 128) router_groups_launch<4>(p, s);
+    else if (E <= 256) router_groups_launch<8>(p, s);
+    else if (E <= 512) router_groups_launch<16>(p, s);
+    else router_groups_launch<32>(p, s);
+    return tb_last_error();
+}
+
+#include "tape.h"
+TB_TAPE_REGISTER(tb_router_groups)

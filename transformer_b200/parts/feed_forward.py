@@ -13,6 +13,7 @@ from ..csrc import lib
 from .base import FEED_FORWARDS, FeedForward, NormTail, ParamDecl, WeightedRows
 from . import linear
 from .linear import bias_glu_matmul, bias_glu_pays, gemm_skinny, grouped_matmul, matmul_nt
+from .routing import check_choice, choose_experts
 
 ROUTER_ROWS_FROM = 256      # above this many tokens the router works on tiles of 16 tokens (tensor cores)
 ROUTER_TAIL_ROWS = 256      # up to this many tokens the norm before the experts also routes
@@ -134,6 +135,9 @@ class MoE(FeedForward):
       also puts the rows in the experts' order), the experts run on those, and their results are summed unweighted.
     * ``scoring`` = "table": no router.  A table (weight ``table``, [vocab, nexp_use] int32, the entries of a row differ)
       gives every token id its experts; every weight is 1 / nexp_use.
+    * ``scoring`` = "grouped": the choice within groups of parts/routing.py: ``scores`` ("softmax", "sigmoid"), ``groups``,
+      ``groups_use``, ``group_top``, ``renorm``, ``weight_scale``, and ``correction`` as the bias.  The router's product leaves
+      its float logits, and one kernel chooses.
     * ``shared_di`` = n: one more expert of width n (weights ``shared_wgu``, ``shared_wd``; ``shared_limit`` and
       ``glu_alpha`` as above), which every token passes; its result is multiplied by sigmoid(gate . x1), one number a
       token (weight ``shared_gate``), and joins the same weighted sum."""
@@ -153,7 +157,7 @@ class MoE(FeedForward):
         if self.R > 1024:
             raise ValueError(f"the routing kernels take up to 1024 experts, got {self.R}")
         self.scoring = params.get("scoring", "kept")
-        if self.scoring not in ("kept", "all", "sigmoid", "table"):
+        if self.scoring not in ("kept", "all", "sigmoid", "table", "grouped"):
             raise ValueError(f"unknown router scoring {self.scoring!r}")
         self.weight_on = params.get("weight_on", "output")
         if self.weight_on not in ("output", "input"):
@@ -161,8 +165,14 @@ class MoE(FeedForward):
         if self.weight_on == "input" and self.identity:
             raise ValueError("pass-through experts and weights on the input are not combined")
         self.correction = bool(params.get("correction", False))
-        if self.correction and self.scoring != "all":
+        if self.correction and self.scoring not in ("all", "grouped"):
             raise ValueError("a correction of the choice goes with scoring 'all'")
+        self.choice = None
+        if self.scoring == "grouped":
+            self.choice = {"scores": params.get("scores", "softmax"), "groups": int(params.get("groups", 1)),
+                           "groups_use": int(params.get("groups_use", 1)), "group_top": int(params.get("group_top", 1))}
+            check_choice(self.R, self.k, **self.choice)
+            self.choice.update(renorm=bool(params.get("renorm", False)), scale=float(params.get("weight_scale", 1.0)))
         limit = params.get("glu_limit")
         self.glu = None if limit is None else (float(params.get("glu_alpha", 1.0)), float(limit))
         self.plain_router = self.scoring == "kept" and not self.identity
@@ -213,6 +223,11 @@ class MoE(FeedForward):
         nt = x1.shape[0]
         idx = ctx.scratch("moe.topk_idx", (nt, self.k), torch.int32)
         w = ctx.scratch("moe.topk_w", (nt, self.k), torch.float32)
+        if self.choice is not None:
+            logits = logits_out if logits_out is not None else ctx.scratch("moe.logits", (nt, self.R), torch.float32)
+            matmul_nt(x1, self.weights["router"], logits)           # float out on both paths
+            choose_experts(logits, idx, w, bias=self.weights.get("correction"), **self.choice)
+            return idx, w, False
         if self.scoring == "all":
             # scores over all outputs, choice with the correction, the block that finishes last builds the lists
             done = ctx.scratch("moe.done", (1,), torch.int32, zero=True) if lists is not None else None
@@ -264,7 +279,7 @@ class MoE(FeedForward):
                             gate=self.weights["shared_gate"] if self.shared else None,
                             index=ctx.scratch("moe.topk_idx", (nt, self.k), torch.int32),
                             scores=ctx.scratch("moe.terms_w", (nt, self.terms), torch.float32))
-        if nt > ROUTER_TAIL_ROWS:
+        if nt > ROUTER_TAIL_ROWS or self.choice is not None:
             return None
         return NormTail("router", weights=self.weights["router"], k=self.k,
                         index=ctx.scratch("moe.topk_idx", (nt, self.k), torch.int32),
