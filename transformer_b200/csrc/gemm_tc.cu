@@ -467,6 +467,19 @@ int make_map(CUtensorMap* out, const void* base, long long rows, int K, long lon
     return 0;
 }
 
+int make_map_3d(CUtensorMap* out, const void* base, long long n0, long long n1, long long n2, long long ld1, long long ld2, int box1,
+                int box2) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return TB_ERR_UNSUPPORTED;
+    cuuint64_t dims[3] = {(cuuint64_t)n0, (cuuint64_t)n1, (cuuint64_t)n2};
+    cuuint64_t strides[2] = {(cuuint64_t)ld1 * 2, (cuuint64_t)ld2 * 2};
+    cuuint32_t box[3] = {TC_BK, (cuuint32_t)box1, (cuuint32_t)box2};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : TB_ERR_ARG;
+}
+
 static __device__ int tc_error_word;
 
 int* tc_error_ptr() {

@@ -319,16 +319,6 @@ __global__ void __launch_bounds__(256) hd_rates_kernel(const float* __restrict__
 }
 
 // ---- launchers ------------------------------------------------------------------------------------------------------
-static int hd_check(const HeadDecayArgs& p) {
-    if (p.nt < 0 || p.B < 0 || p.H <= 0 || p.G <= 0 || p.H % p.G || p.dim <= 0 || p.vdim <= 0 || p.n_slots < 0 ||
-        p.ldq < (long long)p.H * p.dim || p.ldk < (long long)p.G * p.dim || p.ldv < (long long)p.G * p.vdim ||
-        p.ldo < (long long)p.H * p.vdim || (p.gate && p.ldgate < (long long)p.H * p.vdim) || !p.gate != !p.norm ||
-        p.pitch < (long long)p.H * p.dim * p.vdim || p.new_pitch < (long long)p.H * p.dim * p.vdim ||
-        (p.g_stride != 0 && p.g_stride < p.H))
-        return TB_ERR_ARG;
-    if (p.dim > HD_MAX_DIM || p.vdim > HD_MAX_DIM || p.H > 65535) return TB_ERR_UNSUPPORTED;
-    return 0;
-}
 // Four entries of the states an access: rows, heads and slots are whole 16-byte pieces.
 static bool hd_fours(const HeadDecayArgs& p) {
     return p.vdim % 4 == 0 && p.pitch % 4 == 0 && p.new_pitch % 4 == 0 && (((uintptr_t)p.state | (uintptr_t)p.new_state) & 15) == 0;

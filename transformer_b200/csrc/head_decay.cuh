@@ -95,3 +95,15 @@ __device__ __forceinline__ void hd_sums(const HeadDecayArgs& p, int h, int t0, i
         if (i < n) c[i] = HdSum{hi, (float)(x - (double)hi)};
     }
 }
+
+// What every launcher asks of its sizes.
+static inline int hd_check(const HeadDecayArgs& p) {
+    if (p.nt < 0 || p.B < 0 || p.H <= 0 || p.G <= 0 || p.H % p.G || p.dim <= 0 || p.vdim <= 0 || p.n_slots < 0 ||
+        p.ldq < (long long)p.H * p.dim || p.ldk < (long long)p.G * p.dim || p.ldv < (long long)p.G * p.vdim ||
+        p.ldo < (long long)p.H * p.vdim || (p.gate && p.ldgate < (long long)p.H * p.vdim) || !p.gate != !p.norm ||
+        p.pitch < (long long)p.H * p.dim * p.vdim || p.new_pitch < (long long)p.H * p.dim * p.vdim ||
+        (p.g_stride != 0 && p.g_stride < p.H))
+        return TB_ERR_ARG;
+    if (p.dim > HD_MAX_DIM || p.vdim > HD_MAX_DIM || p.H > 65535) return TB_ERR_UNSUPPORTED;
+    return 0;
+}

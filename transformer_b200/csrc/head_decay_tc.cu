@@ -1,0 +1,689 @@
+// Linear attention with one decay for each head (mathematics: head_decay.cuh): prompts in bfloat16 on the tcgen05 tensor cores, key heads of up
+// to 128 entries and value heads of up to 256, in multiples of eight.
+//
+//   hd_update_tc_kernel   a block = a segment x a head: U = K'^T V (dim x vdim, in tensor memory), K'_j = e^{c_L - c_j} k_j
+//   hd_pass_tc_kernel     a thread = four entries of the state of a (sequence, head): walks the segments, leaves S_0 in bfloat16
+//   hd_rows_tc_kernel     a block = 128 tokens of a segment x a head: O = e^{c_i} (Q S_0), then += P V for each 128 keys up to its own,
+//                         P = (Q K^T) e^{c_i - c_j}; with a gate the heads' norm at the end
+//
+// The states stay in float: K' is written as two bfloat16s, the value and what its rounding left (over K and beside it), and both are multiplied
+// with V into the same accumulator, so U is off by 2^-16 of its terms.  P and S_0 enter products whose results are rounded to bfloat16 anyway, and
+// are rounded to it themselves.
+// A factor e^{c_i - c_j} is one exponential for a row and 32 keys times one for a key and the end of its 32, both at most 1; inside
+// the 32 x 32 on the diagonal, where the first would grow, one exponential each.  P takes its place over the scores in tensor memory (the A
+// operand of the second product).  Copies by TMA (3-D maps [tokens, heads, entries]: entries behind a head's are zeros), products issued
+// by one warp, four warps for the rows; two blocks an SM hide each other's waits.  Every wait is bounded.
+#include "head_decay.cuh"
+#include "memory_common.cuh"
+#include "tc_common.cuh"
+
+#define HT_TILE 128
+#define HT_MOST 4               // tiles of a segment
+#define HT_THREADS 192
+#define HT_LOG2E 1.4426950408889634f
+
+struct HdTcArgs {
+    HeadDecayArgs p;
+    __nv_bfloat16* starts;          // [heads of a portion][max_segs][dim][vdim]
+    int* error;
+    int tiles;                      // of a segment: seg / HT_TILE
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ uint64_t ht_desc(uint32_t smem_addr, uint32_t lbo) {     // MN-major: column boxes lbo apart, 8 rows 1024 bytes
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// 16 packed pairs over 16 columns of this thread's lane (tcgen05.wait::st comes before they are handed over)
+__device__ __forceinline__ void ht_store16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void ht_store32(uint32_t taddr, const float (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]),
+        "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]),
+        "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]),
+        "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ float ht_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The decays of a segment's tokens in blocks of 32 (a warp each): e_j = the sum behind token j to its block's end, and the sums before
+// each block in 64 bits, so that no sum of few tokens is a difference of long ones.
+struct alignas(16) HtSums {
+    float e[HT_MOST * HT_TILE];
+    double before[HT_MOST * HT_TILE / 32 + 1];
+};
+// By 128 threads (tid 0..127), which leave together.
+__device__ __forceinline__ void ht_sums(const HeadDecayArgs& p, int h, int t0, int n, int tid, HtSums& s) {
+    const int lane = tid & 31;
+    float x[HT_MOST];
+#pragma unroll
+    for (int u = 0; u < HT_MOST; ++u) {
+        const int i = tid + HT_TILE * u;
+        x[u] = i < n ? hd_log_decay(p.g[(size_t)(p.g_stride ? t0 + i : 0) * p.g_stride + h]) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < HT_MOST; ++u) {
+        if (HT_TILE * u >= n) break;
+        float e = __shfl_down_sync(0xffffffffu, x[u], 1);
+        if (lane == 31) e = 0.f;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const float b = __shfl_down_sync(0xffffffffu, e, o);
+            if (lane + o < 32) e += b;
+        }
+        s.e[tid + HT_TILE * u] = e;
+        if (lane == 0) s.before[(tid >> 5) + 4 * u + 1] = (double)e + (double)x[u];
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (tid == 0) {
+        double run = 0.0;
+        s.before[0] = 0.0;
+        for (int b = 1; b <= (n + 31) / 32; ++b) s.before[b] = run += s.before[b];
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+}
+
+// ---- U of a segment -----------------------------------------------------------------------------------------------------
+template <int KB, int VB>
+__global__ void __launch_bounds__(HT_THREADS, VB == 4 ? 1 : 2)
+hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const HdTcArgs a) {
+    pdl_sync();
+    constexpr int DK = KB * 64, DV = VB * 64;
+    constexpr uint32_t BOX = HT_TILE * 128, K_BYTES = KB * BOX, V_BYTES = VB * BOX, TMEM_COLS = VB == 4 ? 256 : VB * 64;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const HeadDecayArgs& p = a.p;
+    const uint32_t sk = smem_u32(smem_raw), sl = sk + K_BYTES, sv = sl + K_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + 2 * K_BYTES + V_BYTES);
+    HtSums& sums = *reinterpret_cast<HtSums*>(bars + 8);
+    uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 7);
+    const int warp = warp_number(), lane = threadIdx.x & 31;
+    const int h = p.h0 + blockIdx.y;
+    const HdSegment s = hd_find(p, blockIdx.x);
+    if (s.b < 0) return;
+    if (sk & 1023u) {
+        if (threadIdx.x == 0) atomicCAS(a.error, 0, 49);
+        return;
+    }
+    const int tiles = (s.n + HT_TILE - 1) / HT_TILE, kv = h / (p.H / p.G);
+    const uint32_t bar0 = smem_u32(bars), full = bar0, ready = bar0 + 8, empty = bar0 + 16;
+    if (threadIdx.x == 0) {
+        mbar_init(full, 1);
+        mbar_init(ready, 4);
+        mbar_init(empty, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    if (warp == 0) {
+        int issued = 0;
+        for (int j = 0; j < tiles; ++j) {
+            if (j > 0 && !mbar_wait_warp(empty, (j - 1) & 1, a.error, 41)) break;
+            if (elect_one()) {
+                mbar_expect_tx(full, K_BYTES + V_BYTES);
+#pragma unroll
+                for (int b = 0; b < KB; ++b) tma_load_3d(sk + b * BOX, &map_k, full, b * 64, kv, s.t0 + j * HT_TILE);
+#pragma unroll
+                for (int b = 0; b < VB; ++b) tma_load_3d(sv + b * BOX, &map_v, full, b * 64, kv, s.t0 + j * HT_TILE);
+            }
+            __syncwarp();
+            issued = j + 1;
+        }
+        if (*(volatile int*)a.error != 0 && issued) mbar_wait(full, (issued - 1) & 1, a.error, 41);
+    } else if (warp == 1) {
+        // A = K'^T and B = V, both with the tokens along the rows of their tiles (MN-major)
+        const uint32_t idesc = umma_idesc(DK, DV) | (1u << 15) | (1u << 16);
+        for (int j = 0; j < tiles; ++j) {
+            if (!mbar_wait_warp(ready, j & 1, a.error, 42)) break;
+            tc_fence_after();
+            if (elect_one()) {
+                const int steps = (min(HT_TILE, s.n - j * HT_TILE) + 15) / 16;
+                for (int k = 0; k < steps; ++k) {
+                    const uint64_t dv = ht_desc(sv + k * 2048, BOX);
+                    umma_bf16(tmem, ht_desc(sk + k * 2048, BOX), dv, idesc, (j | k) != 0);
+                    umma_bf16(tmem, ht_desc(sl + k * 2048, BOX), dv, idesc, 1);
+                }
+                umma_commit(empty);
+            }
+            __syncwarp();
+        }
+    } else {
+        const int tid = threadIdx.x - 64, quad = warp & 3;
+        ht_sums(p, h, s.t0, s.n, tid, sums);
+        const int blocks = (s.n + 31) / 32;
+        const double end = sums.before[blocks];
+        bool ok = true;
+        for (int j = 0; j < tiles && ok; ++j) {
+            ok = mbar_wait_warp(full, j & 1, a.error, 43);
+            if (!ok) break;
+            const int token = j * HT_TILE + tid;
+            const bool there = token < s.n;
+            const float w = there ? expf(sums.e[token] + (float)(end - sums.before[(token >> 5) + 1])) : 0.f;
+            F2 w2;
+            w2.f = make_float2(w, w);
+            uint8_t* row = smem_raw + tid * 128;
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    uint4* at = reinterpret_cast<uint4*>(row + b * BOX + ((i ^ (tid & 7)) << 4));
+                    const uint4 x = there ? *at : make_uint4(0u, 0u, 0u, 0u);
+                    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        F2 f, g;
+                        f.f = make_float2(__uint_as_float(in[e] << 16), __uint_as_float(in[e] & 0xffff0000u));
+                        f = mul2(f, w2);
+                        const __nv_bfloat162 r = __floats2bfloat162_rn(f.f.x, f.f.y);
+                        hi[e] = *reinterpret_cast<const uint32_t*>(&r);
+                        g.f = make_float2(f.f.x - __uint_as_float(hi[e] << 16), f.f.y - __uint_as_float(hi[e] & 0xffff0000u));
+                        const __nv_bfloat162 q = __floats2bfloat162_rn(g.f.x, g.f.y);
+                        lo[e] = *reinterpret_cast<const uint32_t*>(&q);
+                    }
+                    *at = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(at) + K_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+            if (!there) {           // another sequence's values: 0 times one that is no number would not be 0
+                uint8_t* vr = smem_raw + 2 * K_BYTES + tid * 128;
+#pragma unroll
+                for (int b = 0; b < VB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(vr + b * BOX + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ready) : "memory");
+        }
+        if (ok) ok = mbar_wait_warp(empty, (tiles - 1) & 1, a.error, 44);
+        tc_fence_after();
+        if (ok) {
+            const size_t at = (size_t)blockIdx.y * p.max_segs + blockIdx.x;
+            // accumulators of 64 rows lie in the first 16 lanes of each warp's 32
+            const int r = DK == 128 ? quad * 32 + lane : quad * 16 + lane;
+            const bool mine = r < p.dim && (DK == 128 || lane < 16);
+            float* u = p.work + (at * p.dim + (mine ? r : 0)) * p.vdim;
+#pragma unroll
+            for (int c0 = 0; c0 < DV; c0 += 32) {
+                float o[32];
+                tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + c0, o);
+                if (mine) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        if (c0 + i < p.vdim) *reinterpret_cast<float4*>(u + c0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
+            }
+            if (tid == 0) p.seg_g[at] = (float)end;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+// ---- from segment to segment ------------------------------------------------------------------------------------------------
+// Four entries a thread.
+__global__ void __launch_bounds__(256) hd_pass_tc_kernel(const HdTcArgs a) {
+    pdl_sync();
+    const HeadDecayArgs& p = a.p;
+    const int b = blockIdx.x, h = p.h0 + blockIdx.y, size = p.dim * p.vdim;
+    const int e = (blockIdx.z * 256 + threadIdx.x) * 4;
+    int t0, n, slot;
+    if (!hd_sequence(p, b, t0, n, slot) || e >= size) return;
+    float S[4];
+    dm_load<float, 4>(p.state + (size_t)slot * p.pitch + (size_t)h * size + e, S);
+    const int segs = (n + p.seg - 1) / p.seg;
+    const size_t first = (size_t)blockIdx.y * p.max_segs + t0 / p.seg + b;
+    const float* w = p.work + first * size + e;
+    __nv_bfloat16* st = a.starts + first * size + e;
+    constexpr int U = 4;
+    for (int i0 = 0; i0 < segs; i0 += U) {
+        float u[U][4], d[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (i0 + i < segs) {
+                dm_load<float, 4>(w + (size_t)(i0 + i) * size, u[i]);
+                d[i] = p.seg_g[first + i0 + i];
+            }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (i0 + i < segs) {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(S[0], S[1]), hi = __floats2bfloat162_rn(S[2], S[3]);
+                *reinterpret_cast<uint2*>(st + (size_t)(i0 + i) * size) =
+                    make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+                const float f = expf(d[i]);
+#pragma unroll
+                for (int l = 0; l < 4; ++l) S[l] = S[l] * f + u[i][l];
+            }
+    }
+    dm_store<4>(p.new_state + (size_t)slot * p.new_pitch + (size_t)h * size + e, S);
+}
+
+// ---- outputs -------------------------------------------------------------------------------------------------------------------
+// A weight of 0 times a value that is no number would reach the rows before it: in the 128 keys that a block's rows share such values
+// are made 0 for the product (and the rows of other sequences all of them), and the rows that do see them become NaN at the end.
+// One thread a key.
+template <int VB>
+__device__ __forceinline__ void ht_clear(uint8_t* v, int key, bool there, volatile uint32_t* found) {
+    uint8_t* row = v + key * 128;
+    const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
+    if (!there) {
+#pragma unroll
+        for (int i = 0; i < VB * 8; ++i) *reinterpret_cast<uint4*>(row + (i >> 3) * (HT_TILE * 128) + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        return;
+    }
+    {
+        __nv_bfloat162 sum[4] = {zero, zero, zero, zero};     // of 0 times the entries: 0, or NaN
+#pragma unroll
+        for (int b = 0; b < VB; ++b)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint4 x = *reinterpret_cast<const uint4*>(row + b * (HT_TILE * 128) + ((i ^ (key & 7)) << 4));
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]), zero, sum[e]);
+            }
+        sum[0] = __hadd2(__hadd2(sum[0], sum[1]), __hadd2(sum[2], sum[3]));
+        if ((*reinterpret_cast<const uint32_t*>(&sum[0]) & 0x7fff7fffu) == 0) return;
+        *found = 1;
+    }
+    for (int i = 0; i < VB * 32; ++i) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(row + (i >> 5) * (HT_TILE * 128)) + (i & 31);
+        *w = finite_pair(*w);
+    }
+}
+
+template <int KB, int VB>
+__global__ void __launch_bounds__(HT_THREADS, VB == 4 ? 1 : 2)
+hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_s, const HdTcArgs a) {
+    pdl_sync();
+    constexpr int DK = KB * 64, DV = VB * 64;
+    constexpr uint32_t BOX = HT_TILE * 128, K_BYTES = KB * BOX, V_BYTES = VB * BOX, S_BOX = DK * 128, TMEM_COLS = VB == 4 ? 512 : 256;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const HeadDecayArgs& p = a.p;
+    const uint32_t sq = smem_u32(smem_raw), sk = sq + K_BYTES, sv = sk + K_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + 2 * K_BYTES + V_BYTES);
+    HtSums& sums = *reinterpret_cast<HtSums*>(bars + 12);
+    float* by_key = reinterpret_cast<float*>(&sums + 1);        // e^{e_j}
+    uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 11);
+    volatile uint32_t* cleared = &tmem_slot + 1;
+    const int warp = warp_number(), lane = threadIdx.x & 31;
+    const int h = p.h0 + blockIdx.y, x = blockIdx.x / a.tiles, last = blockIdx.x - x * a.tiles;     // this block's tile of its segment
+    const HdSegment s = hd_find(p, x);
+    if (s.b < 0 || last * HT_TILE >= s.n) return;
+    if (sq & 1023u) {
+        if (threadIdx.x == 0) atomicCAS(a.error, 0, 49);
+        return;
+    }
+    const int q0 = s.t0 + last * HT_TILE, nq = min(HT_TILE, s.n - last * HT_TILE), kv = h / (p.H / p.G);
+    const uint32_t bar0 = smem_u32(bars), q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 16, v_full = bar0 + 24, v_empty = bar0 + 32,
+                   s_full = bar0 + 40, p_ready = bar0 + 48, o_start = bar0 + 56, o_done = bar0 + 64;
+    if (threadIdx.x == 0) {
+        *cleared = 0;
+        mbar_init(q_full, 1);
+        mbar_init(k_full, 1);
+        mbar_init(k_empty, 1);
+        mbar_init(v_full, 1);
+        mbar_init(v_empty, 1);
+        mbar_init(s_full, 1);
+        mbar_init(p_ready, 4);
+        mbar_init(o_start, 1);
+        mbar_init(o_done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_o = tmem_slot, tmem_s = tmem_slot + DV;
+    if (warp == 0) {
+        // what v's place holds first is S_0
+        if (elect_one()) {
+            mbar_expect_tx(q_full, K_BYTES);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) tma_load_3d(sq + b * BOX, &map_q, q_full, b * 64, h, q0);
+            mbar_expect_tx(v_full, VB * S_BOX);
+#pragma unroll
+            for (int b = 0; b < VB; ++b) tma_load_3d(sv + b * S_BOX, &map_s, v_full, b * 64, 0, blockIdx.y * p.max_segs + x);
+            mbar_expect_tx(k_full, K_BYTES);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) tma_load_3d(sk + b * BOX, &map_k, k_full, b * 64, kv, s.t0);
+        }
+        __syncwarp();
+        int k_issued = 1, v_issued = 1;
+        bool ok = true;
+        for (int j = 0; j <= last; ++j) {
+            ok = mbar_wait_warp(v_empty, j & 1, a.error, 45);
+            if (!ok) break;
+            if (elect_one()) {
+                mbar_expect_tx(v_full, V_BYTES);
+#pragma unroll
+                for (int b = 0; b < VB; ++b) tma_load_3d(sv + b * BOX, &map_v, v_full, b * 64, kv, s.t0 + j * HT_TILE);
+            }
+            __syncwarp();
+            v_issued = j + 2;
+            if (j == last) break;
+            ok = mbar_wait_warp(k_empty, j & 1, a.error, 45);
+            if (!ok) break;
+            if (elect_one()) {
+                mbar_expect_tx(k_full, K_BYTES);
+#pragma unroll
+                for (int b = 0; b < KB; ++b) tma_load_3d(sk + b * BOX, &map_k, k_full, b * 64, kv, s.t0 + (j + 1) * HT_TILE);
+            }
+            __syncwarp();
+            k_issued = j + 2;
+        }
+        if (*(volatile int*)a.error != 0) {         // no copy is left under way
+            mbar_wait(q_full, 0, a.error, 45);
+            mbar_wait(k_full, (k_issued - 1) & 1, a.error, 45);
+            mbar_wait(v_full, (v_issued - 1) & 1, a.error, 45);
+        }
+    } else if (warp == 1) {
+        const uint32_t idesc_s = umma_idesc(HT_TILE, HT_TILE), idesc_o = umma_idesc(HT_TILE, DV) | (1u << 16);
+        auto scores = [&]() {
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < DK / 16; ++k)
+                    umma_bf16(tmem_s, umma_desc(sq + (k / 4) * BOX) + 2 * (k % 4), umma_desc(sk + (k / 4) * BOX) + 2 * (k % 4), idesc_s, k != 0);
+                umma_commit(s_full);
+                umma_commit(k_empty);
+            }
+            __syncwarp();
+        };
+        bool ok = mbar_wait_warp(q_full, 0, a.error, 46) && mbar_wait_warp(v_full, 0, a.error, 46);
+        if (ok) {
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < DK / 16; ++k)
+                    umma_bf16(tmem_o, umma_desc(sq + (k / 4) * BOX) + 2 * (k % 4), ht_desc(sv + k * 2048, S_BOX), idesc_o, k != 0);
+                umma_commit(o_start);
+                umma_commit(v_empty);
+            }
+            __syncwarp();
+            ok = mbar_wait_warp(k_full, 0, a.error, 46);
+            if (ok) {
+                tc_fence_after();
+                scores();
+            }
+        }
+        for (int j = 0; j <= last && ok; ++j) {
+            ok = mbar_wait_warp(p_ready, j & 1, a.error, 46) && mbar_wait_warp(v_full, (j + 1) & 1, a.error, 46);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+                const int steps = j < last ? HT_TILE / 16 : (nq + 15) / 16;
+                for (int k = 0; k < steps; ++k) umma_bf16_ts(tmem_o, tmem_s + 8 * k, ht_desc(sv + k * 2048, BOX), idesc_o, 1);
+                umma_commit(v_empty);
+                umma_commit(o_done);
+            }
+            __syncwarp();
+            if (j < last) {         // the next scores go where P is
+                ok = mbar_wait_warp(o_done, j & 1, a.error, 46) && mbar_wait_warp(k_full, (j + 1) & 1, a.error, 46);
+                if (!ok) break;
+                tc_fence_after();
+                scores();
+            }
+        }
+    } else {
+        const int tid = threadIdx.x - 64, quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
+        ht_sums(p, h, s.t0, s.n, tid, sums);
+        const int block = last * 4 + quad;
+        const float e_row = sums.e[last * HT_TILE + row] * HT_LOG2E;
+        const bool in = row < nq;
+#pragma unroll
+        for (int u = 0; u < HT_MOST; ++u)
+            if (u <= last) by_key[tid + HT_TILE * u] = ht_ex2(sums.e[tid + HT_TILE * u] * HT_LOG2E);
+        // the row's sum from its block's start
+        const float l_row = [&] {
+            float v = in ? hd_log_decay(p.g[(size_t)(p.g_stride ? q0 + row : 0) * p.g_stride + h]) : 0.f;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const float u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += u;
+            }
+            return v;
+        }();
+        const double at_block = in ? sums.before[block] : 0.0;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        bool ok = mbar_wait_warp(o_start, 0, a.error, 47);
+        tc_fence_after();
+        if (ok) {
+            const float f = ht_ex2((l_row + (float)at_block) * HT_LOG2E);
+#pragma unroll
+            for (int c0 = 0; c0 < DV; c0 += 32) {
+                float o[32];
+                tmem_ld32(tmem_o + lane_sel + c0, o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] *= f;
+                ht_store32(tmem_o + lane_sel + c0, o);
+            }
+        }
+        for (int j = 0; j <= last && ok; ++j) {
+            ok = mbar_wait_warp(s_full, j & 1, a.error, 47);
+            tc_fence_after();
+            if (!ok) break;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                uint32_t w[16];
+                float v[32];
+                if (j < last || b <= quad) tmem_ld32(tmem_s + lane_sel + 32 * b, v);
+                if (j < last || b < quad) {
+                    F2 f;
+                    const float r = in ? ht_ex2((l_row + (float)(at_block - sums.before[j * 4 + b + 1])) * HT_LOG2E) : 0.f;
+                    f.f = make_float2(r, r);
+                    const float4* fk = reinterpret_cast<const float4*>(by_key + j * HT_TILE + 32 * b);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 y = fk[i];
+                        F2 s0, s1, y0, y1;
+                        s0.f = make_float2(v[4 * i], v[4 * i + 1]);
+                        s1.f = make_float2(v[4 * i + 2], v[4 * i + 3]);
+                        y0.f = make_float2(y.x, y.y);
+                        y1.f = make_float2(y.z, y.w);
+                        s0 = mul2(mul2(s0, f), y0);
+                        s1 = mul2(mul2(s1, f), y1);
+                        const __nv_bfloat162 h0 = __floats2bfloat162_rn(s0.f.x, s0.f.y), h1 = __floats2bfloat162_rn(s1.f.x, s1.f.y);
+                        w[2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
+                        w[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+                    }
+                } else if (b == quad) {
+                    const float4* ek = reinterpret_cast<const float4*>(sums.e + j * HT_TILE + 32 * b);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 y = ek[i];
+                        const float z[4] = {y.x, y.y, y.z, y.w};
+                        float o[4];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) o[c] = 4 * i + c <= lane ? v[4 * i + c] * ht_ex2(fmaf(z[c], HT_LOG2E, -e_row)) : 0.f;
+                        const __nv_bfloat162 h0 = __floats2bfloat162_rn(o[0], o[1]), h1 = __floats2bfloat162_rn(o[2], o[3]);
+                        w[2 * i] = *reinterpret_cast<const uint32_t*>(&h0);
+                        w[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) w[i] = 0u;
+                }
+                ht_store16(tmem_s + lane_sel + 16 * b, w);
+            }
+            if (j == last) {
+                ok = mbar_wait_warp(v_full, (j + 1) & 1, a.error, 47);
+                if (!ok) break;
+                ht_clear<VB>(smem_raw + 2 * K_BYTES, tid, tid < nq, cleared);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(p_ready) : "memory");
+        }
+        if (ok) ok = mbar_wait_warp(o_done, last & 1, a.error, 48);
+        tc_fence_after();
+        asm volatile("bar.sync 1, 128;" ::: "memory");          // *cleared, as any of the four warps left it
+        if (ok) {
+            const bool some = *cleared != 0;
+            const int t = q0 + row;
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (size_t)t * p.ldo + (size_t)h * p.vdim;
+            const __nv_bfloat16* gate = static_cast<const __nv_bfloat16*>(p.gate) + (size_t)t * p.ldgate + (size_t)h * p.vdim;
+            const float* norm = p.norm + (size_t)h * p.vdim;
+            const __nv_bfloat16* seen = static_cast<const __nv_bfloat16*>(p.v) + (size_t)q0 * p.ldv + (size_t)kv * p.vdim;
+            float by = p.scale;
+            bool bad = false;           // one of the row's outputs is no number
+            auto unclear = [&](int c) {
+                for (int k = 0; k <= row; ++k)
+                    if (!(fabsf(__bfloat162float(seen[(size_t)k * p.ldv + c])) < INFINITY)) return true;
+                return false;
+            };
+            if (p.gate) {
+                float sq = 0.f;
+#pragma unroll
+                for (int c0 = 0; c0 < DV; c0 += 32) {
+                    float o[32];
+                    tmem_ld32(tmem_o + lane_sel + c0, o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sq += o[i] * o[i];
+                }
+                if (some && in)
+                    for (int c = 0; c < p.vdim && !bad; ++c) bad = unclear(c);
+                sq *= p.scale * p.scale;
+                by = bad ? __int_as_float(0x7fc00000) : p.scale * rsqrtf(sq / (float)p.vdim + p.eps);
+            }
+#pragma unroll
+            for (int c0 = 0; c0 < DV; c0 += 32) {
+                float o[32];
+                tmem_ld32(tmem_o + lane_sel + c0, o);
+                if (in) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    if (c0 + i >= p.vdim) continue;
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = o[i + e] * by;
+                    if (p.gate) {
+                        float z[8], w[8];
+                        load8(gate + c0 + i, z);
+                        load8(norm + c0 + i, w);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] *= w[e] * __fdividef(z[e], 1.0f + __expf(-z[e]));
+                    } else if (some) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (unclear(c0 + i + e)) y[e] = __int_as_float(0x7fc00000);
+                    }
+                    store8(dst + c0 + i, y);
+                }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem_slot, TMEM_COLS);
+}
+
+// ---- launchers --------------------------------------------------------------------------------------------------------------------
+template <int KB, int VB>
+static void ht_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& ms, const HdTcArgs& a,
+                      cudaStream_t s) {
+    const HeadDecayArgs& p = a.p;
+    const size_t tiles = (2 * KB + VB) * (size_t)HT_TILE * 128;
+    const size_t smem_u = tiles + 8 * 8 + sizeof(HtSums), smem_r = tiles + 12 * 8 + sizeof(HtSums) + HT_MOST * HT_TILE * sizeof(float);
+    static PerDevice allowed_u, allowed_r;
+    tb_allow_smem(allowed_u, (const void*)hd_update_tc_kernel<KB, VB>, smem_u);
+    tb_allow_smem(allowed_r, (const void*)hd_rows_tc_kernel<KB, VB>, smem_r);
+    if (p.nt) TB_LAUNCH((hd_update_tc_kernel<KB, VB>), dim3(p.max_segs, p.heads), HT_THREADS, smem_u, s, mk, mv, a);
+    TB_LAUNCH((hd_pass_tc_kernel), dim3(p.B, p.heads, (p.dim * p.vdim / 4 + 255) / 256), 256, 0, s, a);
+    if (p.nt) TB_LAUNCH((hd_rows_tc_kernel<KB, VB>), dim3(p.max_segs * a.tiles, p.heads), HT_THREADS, smem_r, s, mq, mk, mv, ms, a);
+}
+
+// Floats of scratch a head for segments of `tiles` tiles: U, S_0 (bfloat16) and the segments' decays.
+static long long ht_work(int nt, int B, int dim, int vdim, int tiles) {
+    const long long segs = nt / (tiles * HT_TILE) + B, size = (long long)dim * vdim;
+    return (segs * (size + size / 2) + segs + 3) / 4 * 4;
+}
+
+extern "C" {
+// 0: these kernels do not take such heads.
+long long tb_head_decay_tc_work(int nt, int B, int dim, int vdim, int tiles) {
+    if (dim <= 0 || vdim <= 0 || dim % 8 || vdim % 8 || dim > 128 || vdim > 256 || tiles < 1 || tiles > HT_MOST) return 0;
+    return ht_work(nt, B, dim, vdim, tiles);
+}
+
+int tb_head_decay_tc_bf16(const void* q, const void* k, const void* v, const void* gate, long long ldq, long long ldk, long long ldv,
+                          long long ldgate, const float* g, int g_stride, const float* norm, const float* state, float* new_state,
+                          long long pitch, long long new_pitch, void* out, long long ldo, const int* seq_start, const int* slots,
+                          float* work, int tiles, int heads, int nt, int B, int H, int G, int dim, int vdim, int n_slots, float scale,
+                          float eps, cudaStream_t s) {
+    HdTcArgs a{HeadDecayArgs{q, k, v, gate, g, norm, state, new_state, out, seq_start, slots, work, nullptr, ldq, ldk, ldv, ldgate, ldo,
+                             pitch, new_pitch, g_stride, nt, B, H, G, dim, vdim, n_slots, 0, tiles * HT_TILE, 0, H, scale, eps},
+               nullptr, nullptr, tiles};
+    HeadDecayArgs& p = a.p;
+    const int rc = hd_check(p);
+    if (rc) return rc;
+    if (heads <= 0 || ((uintptr_t)work & 15)) return TB_ERR_ARG;
+    if (!tb_head_decay_tc_work(nt, B, dim, vdim, tiles)) return TB_ERR_UNSUPPORTED;
+    if (ldq % 8 || ldk % 8 || ldv % 8 || ldo % 8 || ldgate % 8 || pitch % 4 || new_pitch % 4 ||
+        (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)gate | (uintptr_t)out | (uintptr_t)state | (uintptr_t)new_state |
+          (uintptr_t)norm) & 15))
+        return TB_ERR_UNSUPPORTED;
+    if (B == 0) return 0;
+    p.max_segs = nt / p.seg + B;
+    if ((long long)p.max_segs * tiles > 0x7fffffffLL) return TB_ERR_UNSUPPORTED;
+    if (heads > H) heads = H;
+    const size_t size = (size_t)dim * vdim, all = (size_t)heads * p.max_segs;
+    a.starts = reinterpret_cast<__nv_bfloat16*>(work + all * size);
+    p.seg_g = work + all * size + all * (size / 2);
+    a.error = tc_error_ptr();
+    if (!a.error) return tb_last_error();
+    const int kb = (dim + 63) / 64, vb = vdim <= 64 ? 1 : vdim <= 128 ? 2 : 4;
+    CUtensorMap mq, mk, mv, ms;
+    const int rows = nt > 0 ? nt : 1;
+    if (make_map_3d(&mq, q, dim, H, rows, dim, ldq, 1, HT_TILE) || make_map_3d(&mk, k, dim, G, rows, dim, ldk, 1, HT_TILE) ||
+        make_map_3d(&mv, v, vdim, G, rows, vdim, ldv, 1, HT_TILE) ||
+        make_map_3d(&ms, a.starts, vdim, dim, (long long)all, vdim, (long long)size, kb * 64, 1))
+        return TB_ERR_UNSUPPORTED;
+    for (p.h0 = 0; p.h0 < H; p.h0 += heads) {
+        p.heads = H - p.h0 < heads ? H - p.h0 : heads;
+        if (kb == 1) {
+            if (vb == 1) ht_launch<1, 1>(mq, mk, mv, ms, a, s);
+            else if (vb == 2) ht_launch<1, 2>(mq, mk, mv, ms, a, s);
+            else ht_launch<1, 4>(mq, mk, mv, ms, a, s);
+        } else {
+            if (vb == 1) ht_launch<2, 1>(mq, mk, mv, ms, a, s);
+            else if (vb == 2) ht_launch<2, 2>(mq, mk, mv, ms, a, s);
+            else ht_launch<2, 4>(mq, mk, mv, ms, a, s);
+        }
+    }
+    return tb_last_error();
+}
+}
+
+#include "tape.h"
+TB_TAPE_REGISTER(tb_head_decay_tc_bf16)

@@ -114,6 +114,7 @@ _SIGNATURES: Dict[str, str] = {
     "tb_post_add_layernorm_router_bf16": "pppppippfipppfipiippppiii",
     "tb_head_decay_f32": "ppppllllpipppllplpppiiiiiiiiiff", "tb_head_decay_bf16": "ppppllllpipppllplpppiiiiiiiiiff",
     "tb_head_decay_step_f32": "ppppllllpipppllplpiiiiiiff", "tb_head_decay_step_bf16": "ppppllllpipppllplpiiiiiiff",
+    "tb_head_decay_tc_bf16": "ppppllllpipppllplpppiiiiiiiiiff",
     "tb_head_decay_rates": "ppppii",
     "tb_router_groups": "plpppiiiiiiiif",
 }
@@ -169,6 +170,8 @@ def library() -> ctypes.CDLL:
                 fn = getattr(lib, name)
                 fn.argtypes = [_CODES[c] for c in codes]
                 fn.restype = _I
+            lib.tb_head_decay_tc_work.argtypes = [_I] * 5
+            lib.tb_head_decay_tc_work.restype = _L
             lib.tb_tape_index.argtypes = [ctypes.c_char_p]
             lib.tb_tape_index.restype = _I
             lib.tb_tape_replay.argtypes = [ctypes.POINTER(TapeEntry), _I, ctypes.POINTER(TapeMap), _I,
@@ -411,7 +414,7 @@ def kernel_status_async(host_int32: torch.Tensor) -> None:
 def _gave_up(code: int) -> str:
     """Which kernel family a wait code belongs to (1..5 tensor-core products, 11..17 tensor-core prompt
     attention, 21..27 decode attention with the page ring, 31..32 the decaying memory's scan, 33..34 the split delta
-    rule's, 35..36 the chunked delta rule's)."""
+    rule's, 35..36 the chunked delta rule's, 41..49 the linear attention with one decay a head)."""
     if 1 <= code <= 5:
         return "tensor-core matrix product"
     if 11 <= code <= 17:
@@ -424,6 +427,8 @@ def _gave_up(code: int) -> str:
         return "scan of the split delta rule"
     if 35 <= code <= 36:
         return "chunk scan of the delta rule"
+    if 41 <= code <= 49:
+        return "linear attention with one decay a head"
     return "unknown kernel"
 
 
@@ -506,6 +511,12 @@ def split_delta_record_size(dim: int) -> int:
 def head_decay_segments(tokens: int, sequences: int) -> int:
     """Segments that a step's tokens are cut into at most, for the linear attention with one decay a head."""
     return library().tb_head_decay_segments(tokens, sequences)
+
+
+def head_decay_tc_work(tokens: int, sequences: int, dim: int, vdim: int, tiles: int) -> int:
+    """Floats of scratch a head for the tcgen05 kernels of that attention, with segments of ``tiles`` times 128 tokens; 0: they do not
+    take such heads."""
+    return library().tb_head_decay_tc_work(tokens, sequences, dim, vdim, tiles)
 
 
 def attention_window_mma_tile_tokens(nh: int, nkvh: int) -> int:

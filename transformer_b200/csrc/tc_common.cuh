@@ -187,5 +187,9 @@ __device__ __forceinline__ uint32_t umma_idesc(int m, int n) {
 // A cached tensor map of a [rows, K] bfloat16 matrix with row pitch ld: box = 64 columns x box_rows
 // rows, 128-byte swizzle.  0 or a TB_ERR_* code.
 int make_map(CUtensorMap* out, const void* base, long long rows, int K, long long ld, int box_rows);
+// A tensor map of a [n2, n1, n0] bfloat16 array with pitches ld2 and ld1: box = 64 x box1 x box2 (innermost first), 128-byte swizzle; what a
+// box has outside the array is zeros.  Not cached.
+int make_map_3d(CUtensorMap* out, const void* base, long long n0, long long n1, long long n2, long long ld1, long long ld2, int box1,
+                int box2);
 // Device address of the error word that bounded waits set (read and cleared by tb_gemm_tc_status).
 int* tc_error_ptr();

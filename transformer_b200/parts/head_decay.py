@@ -18,6 +18,8 @@ from .base import MIXERS, Mixer, ParamDecl, StateNeed
 from .linear import matmul_nt
 
 MOST_DIM = 256                  # entries of a head, key or value
+USE_TC = True                   # bfloat16 prompts: the tcgen05 kernels, for the heads that they take
+TILES = 2                       # tiles of 128 tokens in one of their segments
 WORK_BYTES = 512 << 20          # the most scratch for the segments' states: of more heads than it holds, portions are done in turn
 
 
@@ -100,13 +102,21 @@ def decay_attention(q, k, v, log_decay, state, seq_start, slots, out, *, scale=N
         raise ValueError(f"seq_start must be a contiguous int32 tensor of {B + 1} entries")
     lib.check_device(q, seq_start)
     H, G, dim, vdim, n_slots = sizes
+    more = (*sizes, dim ** -0.5 if scale is None else float(scale), float(eps))
+
+    def work(per):          # scratch for so many heads as WORK_BYTES holds
+        heads = max(1, min(H, WORK_BYTES // (4 * max(per, 1))))
+        n = heads * per
+        return heads, torch.empty(n, dtype=torch.float32, device=q.device) if scratch is None else scratch("head_decay.work", (n,), torch.float32)
+
+    per = lib.head_decay_tc_work(nt, B, dim, vdim, TILES) if q.dtype == torch.bfloat16 and USE_TC else 0
+    if per:
+        heads, w = work(per)
+        if lib.try_call("tb_head_decay_tc_bf16", *head, seq_start.data_ptr(), slots.data_ptr(), w.data_ptr(), TILES, heads, nt, B, *more):
+            return
     segments = lib.head_decay_segments(nt, B)
-    per = segments * (dim * vdim + 1)
-    heads = max(1, min(H, WORK_BYTES // (4 * max(per, 1))))
-    work = torch.empty(heads * per, dtype=torch.float32, device=q.device) if scratch is None else \
-        scratch("head_decay.work", (heads * per,), torch.float32)
-    lib.call("tb_head_decay_" + lib.suffix(q.dtype), *head, seq_start.data_ptr(), slots.data_ptr(), work.data_ptr(), segments, heads, nt, B,
-             *sizes, dim ** -0.5 if scale is None else float(scale), float(eps))
+    heads, w = work(segments * (dim * vdim + 1))
+    lib.call("tb_head_decay_" + lib.suffix(q.dtype), *head, seq_start.data_ptr(), slots.data_ptr(), w.data_ptr(), segments, heads, nt, B, *more)
 
 
 def decay_attention_step(q, k, v, log_decay, state, slots, out, *, scale=None, norm=None, gate=None, eps=1e-6, new_state=None) -> None:
