@@ -25,6 +25,7 @@
 struct HdTcArgs {
     HeadDecayArgs p;
     __nv_bfloat16* starts;          // [heads of a portion][max_segs][dim][vdim]
+    float* sums;                    // [heads of a portion][max_segs][ht_record(seg)]
     int* error;
     int tiles;                      // of a segment: seg / HT_TILE
 };
@@ -69,14 +70,17 @@ __device__ __forceinline__ float ht_ex2(float x) {
     return y;
 }
 
-// The decays of a segment's tokens in blocks of 32 (a warp each): e_j = the sum behind token j to its block's end, and the sums before
-// each block in 64 bits, so that no sum of few tokens is a difference of long ones.
+// The decays of a segment's tokens in blocks of 32: e_j = the sum behind token j to its block's end, l_j = up to and with token j from its
+// block's start, and the sums before each block in 64 bits, so that no sum of few tokens is a difference of long ones.  The blocks that
+// make U leave them in scratch for those that make the outputs: a record of e [seg], l [seg], before.
+#define HT_BLOCKS (HT_MOST * HT_TILE / 32)
 struct alignas(16) HtSums {
     float e[HT_MOST * HT_TILE];
-    double before[HT_MOST * HT_TILE / 32 + 1];
+    double before[HT_BLOCKS + 2];
 };
+__host__ __device__ inline int ht_record(int seg) { return 2 * seg + 2 * (HT_BLOCKS + 2); }
 // By 128 threads (tid 0..127), which leave together.
-__device__ __forceinline__ void ht_sums(const HeadDecayArgs& p, int h, int t0, int n, int tid, HtSums& s) {
+__device__ __forceinline__ void ht_sums(const HeadDecayArgs& p, int h, int t0, int n, int tid, HtSums& s, float* record) {
     const int lane = tid & 31;
     float x[HT_MOST];
 #pragma unroll
@@ -87,26 +91,42 @@ __device__ __forceinline__ void ht_sums(const HeadDecayArgs& p, int h, int t0, i
 #pragma unroll
     for (int u = 0; u < HT_MOST; ++u) {
         if (HT_TILE * u >= n) break;
-        float e = __shfl_down_sync(0xffffffffu, x[u], 1);
+        float l = x[u], e = __shfl_down_sync(0xffffffffu, x[u], 1);
         if (lane == 31) e = 0.f;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const float b = __shfl_down_sync(0xffffffffu, e, o);
+            const float a = __shfl_up_sync(0xffffffffu, l, o), b = __shfl_down_sync(0xffffffffu, e, o);
+            if (lane >= o) l += a;
             if (lane + o < 32) e += b;
         }
         s.e[tid + HT_TILE * u] = e;
-        if (lane == 0) s.before[(tid >> 5) + 4 * u + 1] = (double)e + (double)x[u];
+        record[tid + HT_TILE * u] = e;
+        record[p.seg + tid + HT_TILE * u] = l;
+        if (lane == 31) s.before[(tid >> 5) + 4 * u] = (double)l;
     }
     asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (tid == 0) {
-        double run = 0.0;
-        s.before[0] = 0.0;
-        for (int b = 1; b <= (n + 31) / 32; ++b) s.before[b] = run += s.before[b];
+    if (tid < 32) {         // the blocks' sums, to those before each
+        double v = lane < (n + 31) / 32 ? s.before[lane] : 0.0;
+        const double own = v;
+#pragma unroll
+        for (int o = 1; o < HT_BLOCKS; o <<= 1) {
+            const double a = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += a;
+        }
+        if (lane <= HT_BLOCKS) {
+            s.before[lane] = v - own;
+            reinterpret_cast<double*>(record + 2 * p.seg)[lane] = v - own;
+        }
     }
     asm volatile("bar.sync 1, 128;" ::: "memory");
 }
 
 // ---- U of a segment -----------------------------------------------------------------------------------------------------
+// Shared memory of the tiles K, what rounding left of K' and V, and of U's rows afterwards.
+__host__ __device__ constexpr int ht_update_area(int kb, int vb) {
+    const int tiles = (2 * kb + vb) * HT_TILE * 128, rows = (kb * 64 * (vb * 256 + 16) + 1023) / 1024 * 1024;
+    return tiles > rows ? tiles : rows;
+}
 template <int KB, int VB>
 __global__ void __launch_bounds__(HT_THREADS, VB == 4 ? 1 : 2)
 hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const HdTcArgs a) {
@@ -116,7 +136,7 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const HeadDecayArgs& p = a.p;
     const uint32_t sk = smem_u32(smem_raw), sl = sk + K_BYTES, sv = sl + K_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + 2 * K_BYTES + V_BYTES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + ht_update_area(KB, VB));
     HtSums& sums = *reinterpret_cast<HtSums*>(bars + 8);
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 7);
     const int warp = warp_number(), lane = threadIdx.x & 31;
@@ -174,7 +194,8 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
     } else {
         const int tid = threadIdx.x - 64, quad = warp & 3;
-        ht_sums(p, h, s.t0, s.n, tid, sums);
+        const size_t at = (size_t)blockIdx.y * p.max_segs + blockIdx.x;
+        ht_sums(p, h, s.t0, s.n, tid, sums, a.sums + at * ht_record(p.seg));
         const int blocks = (s.n + 31) / 32;
         const double end = sums.before[blocks];
         bool ok = true;
@@ -187,9 +208,9 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             F2 w2;
             w2.f = make_float2(w, w);
             uint8_t* row = smem_raw + tid * 128;
-#pragma unroll
+#pragma unroll 1
             for (int b = 0; b < KB; ++b)
-#pragma unroll
+#pragma unroll 4
                 for (int i = 0; i < 8; ++i) {
                     uint4* at = reinterpret_cast<uint4*>(row + b * BOX + ((i ^ (tid & 7)) << 4));
                     const uint4 x = there ? *at : make_uint4(0u, 0u, 0u, 0u);
@@ -223,20 +244,27 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (ok) ok = mbar_wait_warp(empty, (tiles - 1) & 1, a.error, 44);
         tc_fence_after();
         if (ok) {
-            const size_t at = (size_t)blockIdx.y * p.max_segs + blockIdx.x;
-            // accumulators of 64 rows lie in the first 16 lanes of each warp's 32
+            // accumulators of 64 rows lie in the first 16 lanes of each warp's 32.  A row goes through shared memory (free by now) and leaves
+            // as one bulk copy; rows 16 bytes more than their entries apart, so that lanes do not meet in the banks
             const int r = DK == 128 ? quad * 32 + lane : quad * 16 + lane;
             const bool mine = r < p.dim && (DK == 128 || lane < 16);
-            float* u = p.work + (at * p.dim + (mine ? r : 0)) * p.vdim;
-#pragma unroll
+            uint8_t* stage = smem_raw + r * (DV * 4 + 16);
+#pragma unroll 1
             for (int c0 = 0; c0 < DV; c0 += 32) {
                 float o[32];
                 tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + c0, o);
                 if (mine) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        if (c0 + i < p.vdim) *reinterpret_cast<float4*>(u + c0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        *reinterpret_cast<float4*>(stage + (c0 + i) * 4) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 }
+            }
+            if (mine) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.work + (at * p.dim + r) * p.vdim),
+                             "r"(smem_u32(stage)), "r"(p.vdim * 4) : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
             }
             if (tid == 0) p.seg_g[at] = (float)end;
         }
@@ -318,19 +346,41 @@ __device__ __forceinline__ void ht_clear(uint8_t* v, int key, bool there, volati
     }
 }
 
+// The row's outputs in the channels where one of the block's tokens up to its own has a value that is no number (gated: all of them, through
+// the norm); `seen`: the block's values.
+__device__ __noinline__ void ht_unclear(const __nv_bfloat16* seen, long long ldv, int vdim, int row, bool all, uint8_t* mine) {
+    bool any = false;
+    for (int pass = 0; pass < (all ? 2 : 1); ++pass)
+        for (int c = 0; c < vdim; ++c) {
+            bool bad = pass == 1 && any;
+            for (int k = 0; k <= row && !bad; ++k) bad = !(fabsf(__bfloat162float(seen[(size_t)k * ldv + c])) < INFINITY);
+            any = any || bad;
+            if (bad)
+                *reinterpret_cast<uint16_t*>(mine + (c >> 6) * (HT_TILE * 128) + ((((c & 63) >> 3) ^ (row & 7)) << 4) + (c & 7) * 2) = 0x7fff;
+        }
+}
+
+struct alignas(16) HtRowsShared {
+    float e[HT_MOST * HT_TILE], by_key[HT_MOST * HT_TILE];       // e_j and e^{e_j}
+    float norm[256];
+    double before[HT_BLOCKS + 2];
+};
+
 template <int KB, int VB>
 __global__ void __launch_bounds__(HT_THREADS, VB == 4 ? 1 : 2)
 hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_s, const HdTcArgs a) {
+                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_s,
+                  const __grid_constant__ CUtensorMap map_g, const HdTcArgs a) {
     pdl_sync();
     constexpr int DK = KB * 64, DV = VB * 64;
     constexpr uint32_t BOX = HT_TILE * 128, K_BYTES = KB * BOX, V_BYTES = VB * BOX, S_BOX = DK * 128, TMEM_COLS = VB == 4 ? 512 : 256;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const HeadDecayArgs& p = a.p;
-    const uint32_t sq = smem_u32(smem_raw), sk = sq + K_BYTES, sv = sk + K_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + 2 * K_BYTES + V_BYTES);
-    HtSums& sums = *reinterpret_cast<HtSums*>(bars + 12);
-    float* by_key = reinterpret_cast<float*>(&sums + 1);        // e^{e_j}
+    // Q and K, and once no product reads them the gate's tile, in whose place the outputs are staged
+    constexpr uint32_t QK_BYTES = (2 * KB > VB ? 2 * KB : VB) * BOX;
+    const uint32_t sq = smem_u32(smem_raw), sk = sq + K_BYTES, sv = sq + QK_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + QK_BYTES + V_BYTES);
+    HtRowsShared& sh = *reinterpret_cast<HtRowsShared*>(bars + 12);
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 11);
     volatile uint32_t* cleared = &tmem_slot + 1;
     const int warp = warp_number(), lane = threadIdx.x & 31;
@@ -343,7 +393,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     }
     const int q0 = s.t0 + last * HT_TILE, nq = min(HT_TILE, s.n - last * HT_TILE), kv = h / (p.H / p.G);
     const uint32_t bar0 = smem_u32(bars), q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 16, v_full = bar0 + 24, v_empty = bar0 + 32,
-                   s_full = bar0 + 40, p_ready = bar0 + 48, o_start = bar0 + 56, o_done = bar0 + 64;
+                   s_full = bar0 + 40, p_ready = bar0 + 48, o_start = bar0 + 56, o_done = bar0 + 64, g_full = bar0 + 72;
     if (threadIdx.x == 0) {
         *cleared = 0;
         mbar_init(q_full, 1);
@@ -355,6 +405,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         mbar_init(p_ready, 4);
         mbar_init(o_start, 1);
         mbar_init(o_done, 1);
+        mbar_init(g_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
@@ -377,7 +428,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         __syncwarp();
         int k_issued = 1, v_issued = 1;
-        bool ok = true;
+        bool ok = true, gate_issued = false;
         for (int j = 0; j <= last; ++j) {
             ok = mbar_wait_warp(v_empty, j & 1, a.error, 45);
             if (!ok) break;
@@ -388,9 +439,19 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             }
             __syncwarp();
             v_issued = j + 2;
-            if (j == last) break;
+            if (j == last && !p.gate) break;
             ok = mbar_wait_warp(k_empty, j & 1, a.error, 45);
             if (!ok) break;
+            if (j == last) {
+                if (elect_one()) {
+                    mbar_expect_tx(g_full, V_BYTES);
+#pragma unroll
+                    for (int b = 0; b < VB; ++b) tma_load_3d(sq + b * BOX, &map_g, g_full, b * 64, h, q0);
+                }
+                __syncwarp();
+                gate_issued = true;
+                break;
+            }
             if (elect_one()) {
                 mbar_expect_tx(k_full, K_BYTES);
 #pragma unroll
@@ -403,6 +464,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             mbar_wait(q_full, 0, a.error, 45);
             mbar_wait(k_full, (k_issued - 1) & 1, a.error, 45);
             mbar_wait(v_full, (v_issued - 1) & 1, a.error, 45);
+            if (gate_issued) mbar_wait(g_full, 0, a.error, 45);
         }
     } else if (warp == 1) {
         const uint32_t idesc_s = umma_idesc(HT_TILE, HT_TILE), idesc_o = umma_idesc(HT_TILE, DV) | (1u << 16);
@@ -454,30 +516,25 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     } else {
         const int tid = threadIdx.x - 64, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
-        ht_sums(p, h, s.t0, s.n, tid, sums);
-        const int block = last * 4 + quad;
-        const float e_row = sums.e[last * HT_TILE + row] * HT_LOG2E;
+        const float* record = a.sums + ((size_t)blockIdx.y * p.max_segs + x) * ht_record(p.seg);
         const bool in = row < nq;
-#pragma unroll
-        for (int u = 0; u < HT_MOST; ++u)
-            if (u <= last) by_key[tid + HT_TILE * u] = ht_ex2(sums.e[tid + HT_TILE * u] * HT_LOG2E);
-        // the row's sum from its block's start
-        const float l_row = [&] {
-            float v = in ? hd_log_decay(p.g[(size_t)(p.g_stride ? q0 + row : 0) * p.g_stride + h]) : 0.f;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const float u = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += u;
-            }
-            return v;
-        }();
-        const double at_block = in ? sums.before[block] : 0.0;
+        const int block = last * 4 + quad;
+        const float e_row = record[last * HT_TILE + row] * HT_LOG2E, l_row = record[p.seg + last * HT_TILE + row];
+        for (int u = tid; u < (last + 1) * HT_TILE; u += HT_TILE) {
+            const float e = record[u];
+            sh.e[u] = e;
+            sh.by_key[u] = ht_ex2(e * HT_LOG2E);
+        }
+        if (tid <= HT_BLOCKS) sh.before[tid] = reinterpret_cast<const double*>(record + 2 * p.seg)[tid];
+        if (p.gate)
+            for (int c = tid; c < p.vdim; c += HT_TILE) sh.norm[c] = p.norm[(size_t)h * p.vdim + c];
         asm volatile("bar.sync 1, 128;" ::: "memory");
+        const double at_block = sh.before[block];
         bool ok = mbar_wait_warp(o_start, 0, a.error, 47);
         tc_fence_after();
         if (ok) {
             const float f = ht_ex2((l_row + (float)at_block) * HT_LOG2E);
-#pragma unroll
+#pragma unroll 1
             for (int c0 = 0; c0 < DV; c0 += 32) {
                 float o[32];
                 tmem_ld32(tmem_o + lane_sel + c0, o);
@@ -490,16 +547,16 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             ok = mbar_wait_warp(s_full, j & 1, a.error, 47);
             tc_fence_after();
             if (!ok) break;
-#pragma unroll
+#pragma unroll 1
             for (int b = 0; b < 4; ++b) {
                 uint32_t w[16];
                 float v[32];
                 if (j < last || b <= quad) tmem_ld32(tmem_s + lane_sel + 32 * b, v);
                 if (j < last || b < quad) {
                     F2 f;
-                    const float r = in ? ht_ex2((l_row + (float)(at_block - sums.before[j * 4 + b + 1])) * HT_LOG2E) : 0.f;
+                    const float r = in ? ht_ex2((l_row + (float)(at_block - sh.before[j * 4 + b + 1])) * HT_LOG2E) : 0.f;
                     f.f = make_float2(r, r);
-                    const float4* fk = reinterpret_cast<const float4*>(by_key + j * HT_TILE + 32 * b);
+                    const float4* fk = reinterpret_cast<const float4*>(sh.by_key + j * HT_TILE + 32 * b);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float4 y = fk[i];
@@ -515,7 +572,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                         w[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&h1);
                     }
                 } else if (b == quad) {
-                    const float4* ek = reinterpret_cast<const float4*>(sums.e + j * HT_TILE + 32 * b);
+                    const float4* ek = reinterpret_cast<const float4*>(sh.e + j * HT_TILE + 32 * b);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float4 y = ek[i];
@@ -536,7 +593,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             if (j == last) {
                 ok = mbar_wait_warp(v_full, (j + 1) & 1, a.error, 47);
                 if (!ok) break;
-                ht_clear<VB>(smem_raw + 2 * K_BYTES, tid, tid < nq, cleared);
+                ht_clear<VB>(smem_raw + QK_BYTES, tid, tid < nq, cleared);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -547,59 +604,54 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (ok) ok = mbar_wait_warp(o_done, last & 1, a.error, 48);
         tc_fence_after();
         asm volatile("bar.sync 1, 128;" ::: "memory");          // *cleared, as any of the four warps left it
+        if (ok && p.gate) ok = mbar_wait_warp(g_full, 0, a.error, 48);
         if (ok) {
-            const bool some = *cleared != 0;
-            const int t = q0 + row;
-            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (size_t)t * p.ldo + (size_t)h * p.vdim;
-            const __nv_bfloat16* gate = static_cast<const __nv_bfloat16*>(p.gate) + (size_t)t * p.ldgate + (size_t)h * p.vdim;
-            const float* norm = p.norm + (size_t)h * p.vdim;
-            const __nv_bfloat16* seen = static_cast<const __nv_bfloat16*>(p.v) + (size_t)q0 * p.ldv + (size_t)kv * p.vdim;
             float by = p.scale;
-            bool bad = false;           // one of the row's outputs is no number
-            auto unclear = [&](int c) {
-                for (int k = 0; k <= row; ++k)
-                    if (!(fabsf(__bfloat162float(seen[(size_t)k * p.ldv + c])) < INFINITY)) return true;
-                return false;
-            };
             if (p.gate) {
-                float sq = 0.f;
-#pragma unroll
+                float sq2 = 0.f;
+#pragma unroll 1
                 for (int c0 = 0; c0 < DV; c0 += 32) {
                     float o[32];
                     tmem_ld32(tmem_o + lane_sel + c0, o);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sq += o[i] * o[i];
+                    for (int i = 0; i < 32; ++i) sq2 += o[i] * o[i];
                 }
-                if (some && in)
-                    for (int c = 0; c < p.vdim && !bad; ++c) bad = unclear(c);
-                sq *= p.scale * p.scale;
-                by = bad ? __int_as_float(0x7fc00000) : p.scale * rsqrtf(sq / (float)p.vdim + p.eps);
+                by *= rsqrtf(sq2 * (p.scale * p.scale) / (float)p.vdim + p.eps);
             }
-#pragma unroll
+            // the row's outputs go where its gate is (16-byte pieces in the order of the TMA's swizzle) ...
+            uint8_t* mine = smem_raw + row * 128;
+#pragma unroll 1
             for (int c0 = 0; c0 < DV; c0 += 32) {
                 float o[32];
                 tmem_ld32(tmem_o + lane_sel + c0, o);
-                if (in) {
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
-                    if (c0 + i >= p.vdim) continue;
+                    uint8_t* at = mine + (c0 >> 6) * BOX + (((((c0 & 32) + i) >> 3) ^ (row & 7)) << 4);
                     float y[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) y[e] = o[i + e] * by;
                     if (p.gate) {
-                        float z[8], w[8];
-                        load8(gate + c0 + i, z);
-                        load8(norm + c0 + i, w);
+                        float z[8];
+                        Vec16<__nv_bfloat16>::unpack(*reinterpret_cast<const uint4*>(at), z);
+                        const float4 w0 = *reinterpret_cast<const float4*>(sh.norm + c0 + i), w1 = *reinterpret_cast<const float4*>(sh.norm + c0 + i + 4);
+                        const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
                         for (int e = 0; e < 8; ++e) y[e] *= w[e] * __fdividef(z[e], 1.0f + __expf(-z[e]));
-                    } else if (some) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (unclear(c0 + i + e)) y[e] = __int_as_float(0x7fc00000);
                     }
-                    store8(dst + c0 + i, y);
+                    store8(reinterpret_cast<__nv_bfloat16*>(at), y);
                 }
-                }
+            }
+            if (*cleared && in)
+                ht_unclear(static_cast<const __nv_bfloat16*>(p.v) + (size_t)q0 * p.ldv + (size_t)kv * p.vdim, p.ldv, p.vdim, row, p.gate != nullptr, mine);
+            __syncwarp();
+            // ... and leave in whole lines, the warp's rows one after the other
+            const int pieces = p.vdim >> 3, rows = min(32, nq - quad * 32);
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (size_t)(q0 + quad * 32) * p.ldo + (size_t)h * p.vdim;
+#pragma unroll 4
+            for (int i = lane; i < rows * pieces; i += 32) {
+                const int r = i / pieces, c = i - r * pieces, rr = quad * 32 + r;
+                const uint4 y = *reinterpret_cast<const uint4*>(smem_raw + rr * 128 + (c >> 3) * BOX + (((c & 7) ^ (rr & 7)) << 4));
+                *reinterpret_cast<uint4*>(dst + (size_t)r * p.ldo + c * 8) = y;
             }
         }
     }
@@ -610,23 +662,23 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 
 // ---- launchers --------------------------------------------------------------------------------------------------------------------
 template <int KB, int VB>
-static void ht_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& ms, const HdTcArgs& a,
-                      cudaStream_t s) {
+static void ht_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& ms, const CUtensorMap& mg,
+                      const HdTcArgs& a, cudaStream_t s) {
     const HeadDecayArgs& p = a.p;
-    const size_t tiles = (2 * KB + VB) * (size_t)HT_TILE * 128;
-    const size_t smem_u = tiles + 8 * 8 + sizeof(HtSums), smem_r = tiles + 12 * 8 + sizeof(HtSums) + HT_MOST * HT_TILE * sizeof(float);
+    const size_t box = (size_t)HT_TILE * 128, smem_u = ht_update_area(KB, VB) + 8 * 8 + sizeof(HtSums),
+                 smem_r = ((2 * KB > VB ? 2 * KB : VB) + VB) * box + 12 * 8 + sizeof(HtRowsShared);
     static PerDevice allowed_u, allowed_r;
     tb_allow_smem(allowed_u, (const void*)hd_update_tc_kernel<KB, VB>, smem_u);
     tb_allow_smem(allowed_r, (const void*)hd_rows_tc_kernel<KB, VB>, smem_r);
     if (p.nt) TB_LAUNCH((hd_update_tc_kernel<KB, VB>), dim3(p.max_segs, p.heads), HT_THREADS, smem_u, s, mk, mv, a);
     TB_LAUNCH((hd_pass_tc_kernel), dim3(p.B, p.heads, (p.dim * p.vdim / 4 + 255) / 256), 256, 0, s, a);
-    if (p.nt) TB_LAUNCH((hd_rows_tc_kernel<KB, VB>), dim3(p.max_segs * a.tiles, p.heads), HT_THREADS, smem_r, s, mq, mk, mv, ms, a);
+    if (p.nt) TB_LAUNCH((hd_rows_tc_kernel<KB, VB>), dim3(p.max_segs * a.tiles, p.heads), HT_THREADS, smem_r, s, mq, mk, mv, ms, mg, a);
 }
 
-// Floats of scratch a head for segments of `tiles` tiles: U, S_0 (bfloat16) and the segments' decays.
+// Floats of scratch a head for segments of `tiles` tiles: U, S_0 (bfloat16), the tokens' decays and the segments'.
 static long long ht_work(int nt, int B, int dim, int vdim, int tiles) {
     const long long segs = nt / (tiles * HT_TILE) + B, size = (long long)dim * vdim;
-    return (segs * (size + size / 2) + segs + 3) / 4 * 4;
+    return (segs * (size + size / 2 + ht_record(tiles * HT_TILE)) + segs + 3) / 4 * 4;
 }
 
 extern "C" {
@@ -643,7 +695,7 @@ int tb_head_decay_tc_bf16(const void* q, const void* k, const void* v, const voi
                           float eps, cudaStream_t s) {
     HdTcArgs a{HeadDecayArgs{q, k, v, gate, g, norm, state, new_state, out, seq_start, slots, work, nullptr, ldq, ldk, ldv, ldgate, ldo,
                              pitch, new_pitch, g_stride, nt, B, H, G, dim, vdim, n_slots, 0, tiles * HT_TILE, 0, H, scale, eps},
-               nullptr, nullptr, tiles};
+               nullptr, nullptr, nullptr, tiles};
     HeadDecayArgs& p = a.p;
     const int rc = hd_check(p);
     if (rc) return rc;
@@ -659,26 +711,28 @@ int tb_head_decay_tc_bf16(const void* q, const void* k, const void* v, const voi
     if (heads > H) heads = H;
     const size_t size = (size_t)dim * vdim, all = (size_t)heads * p.max_segs;
     a.starts = reinterpret_cast<__nv_bfloat16*>(work + all * size);
-    p.seg_g = work + all * size + all * (size / 2);
+    a.sums = work + all * size + all * (size / 2);
+    p.seg_g = a.sums + all * ht_record(p.seg);
     a.error = tc_error_ptr();
     if (!a.error) return tb_last_error();
     const int kb = (dim + 63) / 64, vb = vdim <= 64 ? 1 : vdim <= 128 ? 2 : 4;
-    CUtensorMap mq, mk, mv, ms;
+    CUtensorMap mq, mk, mv, ms, mg = {};
     const int rows = nt > 0 ? nt : 1;
     if (make_map_3d(&mq, q, dim, H, rows, dim, ldq, 1, HT_TILE) || make_map_3d(&mk, k, dim, G, rows, dim, ldk, 1, HT_TILE) ||
         make_map_3d(&mv, v, vdim, G, rows, vdim, ldv, 1, HT_TILE) ||
-        make_map_3d(&ms, a.starts, vdim, dim, (long long)all, vdim, (long long)size, kb * 64, 1))
+        make_map_3d(&ms, a.starts, vdim, dim, (long long)all, vdim, (long long)size, kb * 64, 1) ||
+        (gate && make_map_3d(&mg, gate, vdim, H, rows, vdim, ldgate, 1, HT_TILE)))
         return TB_ERR_UNSUPPORTED;
     for (p.h0 = 0; p.h0 < H; p.h0 += heads) {
         p.heads = H - p.h0 < heads ? H - p.h0 : heads;
         if (kb == 1) {
-            if (vb == 1) ht_launch<1, 1>(mq, mk, mv, ms, a, s);
-            else if (vb == 2) ht_launch<1, 2>(mq, mk, mv, ms, a, s);
-            else ht_launch<1, 4>(mq, mk, mv, ms, a, s);
+            if (vb == 1) ht_launch<1, 1>(mq, mk, mv, ms, mg, a, s);
+            else if (vb == 2) ht_launch<1, 2>(mq, mk, mv, ms, mg, a, s);
+            else ht_launch<1, 4>(mq, mk, mv, ms, mg, a, s);
         } else {
-            if (vb == 1) ht_launch<2, 1>(mq, mk, mv, ms, a, s);
-            else if (vb == 2) ht_launch<2, 2>(mq, mk, mv, ms, a, s);
-            else ht_launch<2, 4>(mq, mk, mv, ms, a, s);
+            if (vb == 1) ht_launch<2, 1>(mq, mk, mv, ms, mg, a, s);
+            else if (vb == 2) ht_launch<2, 2>(mq, mk, mv, ms, mg, a, s);
+            else ht_launch<2, 4>(mq, mk, mv, ms, mg, a, s);
         }
     }
     return tb_last_error();
