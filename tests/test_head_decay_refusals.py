@@ -64,7 +64,7 @@ def test_the_choice_refuses(change, what):
 
 def test_more_choices_than_the_kernel_takes():
     with pytest.raises(ValueError, match="per token"):
-        choose_experts(torch.zeros(5, 64), torch.zeros(5, 32, dtype=torch.int32), torch.zeros(5, 32))
+        choose_experts(torch.zeros(5, 64), torch.zeros(5, 31, dtype=torch.int32), torch.zeros(5, 31))
 
 
 MIXER = dict(width=32, heads=4, kv_heads=2, dim=8, vdim=12, eps=1e-6)

@@ -12,6 +12,8 @@
 #include "memory_common.cuh"
 
 #define HD_SEG 64
+#define HD_STEP_NT 256
+#define HD_STEP_U 16
 #define HD_PAD 68               // pitch of a tile of 64 columns
 
 // ---- U of a segment ----------------------------------------------------------------------------------------------
@@ -232,18 +234,17 @@ __global__ void __launch_bounds__(256) hd_rows_kernel(const HeadDecayArgs p) {
 }
 
 // ---- one token per sequence ---------------------------------------------------------------------------------------
-// V: columns a thread and access (four where rows and heads are whole 16-byte pieces).
-template <typename T, int V>
-__global__ void __launch_bounds__(256) hd_step_kernel(const HeadDecayArgs p) {
-    constexpr int U = 8;                    // rows asked for together
+// V: columns a thread and access (four where rows and heads are whole 16-byte pieces); NT threads, U rows asked for together.
+template <typename T, int V, int NT, int U>
+__global__ void __launch_bounds__(NT) hd_step_kernel(const HeadDecayArgs p) {
     extern __shared__ __align__(16) float hd_sm[];
     __shared__ float red[33];
     const int b = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, dim = p.dim, vdim = p.vdim;
-    const int nc = vdim / V, R = 256 / nc;  // columns' threads, groups of rows
+    const int nc = vdim / V, R = NT / nc;   // columns' threads, groups of rows
     const int vp = (vdim + 3) / 4 * 4;
     float* q_s = hd_sm;                     // [dim] each
     float* k_s = q_s + dim;
-    float* o_s = k_s + dim;                 // [R][vp]
+    float* o_s = hd_sm + (2 * dim + 3) / 4 * 4;     // [R][vp]
     pdl_sync();
     const int slot = p.slots[b];
     if (slot < 0 || slot >= p.n_slots) return;
@@ -254,7 +255,15 @@ __global__ void __launch_bounds__(256) hd_step_kernel(const HeadDecayArgs p) {
     auto fetch = [&](int r0) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (r0 + u * R < dim) dm_load<float, V>(S + (size_t)(r0 + u * R) * vdim + c, s[u]);
+            if (r0 + u * R < dim) {
+                const float* at = S + (size_t)(r0 + u * R) * vdim + c;
+                if constexpr (V == 4) {
+                    const float4 f = __ldcs(reinterpret_cast<const float4*>(at));       // read once
+                    s[u][0] = f.x; s[u][1] = f.y; s[u][2] = f.z; s[u][3] = f.w;
+                } else {
+                    s[u][0] = __ldcs(at);
+                }
+            }
     };
     if (rg < R) fetch(rg);
     const int kv = h / (p.H / p.G);
@@ -291,7 +300,9 @@ __global__ void __launch_bounds__(256) hd_step_kernel(const HeadDecayArgs p) {
                     s[u][e] = s[u][e] * decay + kk * v[e];
                     acc[e] += s[u][e] * qq;
                 }
-                dm_store<V>(N + (size_t)r * vdim + c, s[u]);
+                float* at = N + (size_t)r * vdim + c;
+                if constexpr (V == 4) __stcs(reinterpret_cast<float4*>(at), make_float4(s[u][0], s[u][1], s[u][2], s[u][3]));
+                else __stcs(at, s[u][0]);
             }
         }
 #pragma unroll
@@ -364,10 +375,11 @@ static int hd_step_launch(const HeadDecayArgs& p, cudaStream_t s) {
     if (rc) return rc;
     if (p.B == 0) return 0;
     const bool four = hd_fours(p);
-    const int R = 256 / (p.vdim / (four ? 4 : 1)), vp = (p.vdim + 3) / 4 * 4;
-    const size_t smem = (2 * (size_t)p.dim + (size_t)R * vp) * sizeof(float);
-    if (four) TB_LAUNCH((hd_step_kernel<T, 4>), dim3(p.B, p.H), 256, smem, s, p);
-    else TB_LAUNCH((hd_step_kernel<T, 1>), dim3(p.B, p.H), 256, smem, s, p);
+    constexpr int NT = HD_STEP_NT;
+    const int R = NT / (p.vdim / (four ? 4 : 1)), vp = (p.vdim + 3) / 4 * 4;
+    const size_t smem = ((2 * (size_t)p.dim + 3) / 4 * 4 + (size_t)R * vp) * sizeof(float);
+    if (four) TB_LAUNCH((hd_step_kernel<T, 4, NT, HD_STEP_U>), dim3(p.B, p.H), NT, smem, s, p);
+    else TB_LAUNCH((hd_step_kernel<T, 1, NT, HD_STEP_U>), dim3(p.B, p.H), NT, smem, s, p);
     return tb_last_error();
 }
 

@@ -19,7 +19,8 @@
 
 #define HT_TILE 128
 #define HT_MOST 4               // tiles of a segment
-#define HT_THREADS 192
+#define HT_WORKERS 256          // eight warps: two for each 32 lanes of tensor memory, half of the columns each
+#define HT_THREADS (64 + HT_WORKERS)
 #define HT_LOG2E 1.4426950408889634f
 
 struct HdTcArgs {
@@ -79,19 +80,17 @@ struct alignas(16) HtSums {
     double before[HT_BLOCKS + 2];
 };
 __host__ __device__ inline int ht_record(int seg) { return 2 * seg + 2 * (HT_BLOCKS + 2); }
-// By 128 threads (tid 0..127), which leave together.
-__device__ __forceinline__ void ht_sums(const HeadDecayArgs& p, int h, int t0, int n, int tid, HtSums& s, float* record) {
+// By the workers (tid 0..255), which leave together.
+__device__ __forceinline__ void ht_sums(const HeadDecayArgs& p, int h, int t0, int n, int tid, HtSums& s, float* __restrict__ record) {
+    constexpr int U = HT_MOST * HT_TILE / HT_WORKERS;
     const int lane = tid & 31;
-    float x[HT_MOST];
+    float x[U];
 #pragma unroll
-    for (int u = 0; u < HT_MOST; ++u) {
-        const int i = tid + HT_TILE * u;
-        x[u] = i < n ? hd_log_decay(p.g[(size_t)(p.g_stride ? t0 + i : 0) * p.g_stride + h]) : 0.f;
-    }
+    for (int u = 0; u < U; ++u) x[u] = p.g[(size_t)(p.g_stride ? t0 + min(tid + HT_WORKERS * u, n - 1) : 0) * p.g_stride + h];
 #pragma unroll
-    for (int u = 0; u < HT_MOST; ++u) {
-        if (HT_TILE * u >= n) break;
-        float l = x[u], e = __shfl_down_sync(0xffffffffu, x[u], 1);
+    for (int u = 0; u < U; ++u) {
+        const int i = tid + HT_WORKERS * u;
+        float l = i < n ? hd_log_decay(x[u]) : 0.f, e = __shfl_down_sync(0xffffffffu, l, 1);
         if (lane == 31) e = 0.f;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -99,26 +98,28 @@ __device__ __forceinline__ void ht_sums(const HeadDecayArgs& p, int h, int t0, i
             if (lane >= o) l += a;
             if (lane + o < 32) e += b;
         }
-        s.e[tid + HT_TILE * u] = e;
-        record[tid + HT_TILE * u] = e;
-        record[p.seg + tid + HT_TILE * u] = l;
-        if (lane == 31) s.before[(tid >> 5) + 4 * u] = (double)l;
+        s.e[i] = e;
+        if (lane == 31) s.before[i >> 5] = (double)l;
+        if (i < p.seg) {
+            record[i] = e;
+            record[p.seg + i] = l;
+        }
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    asm volatile("bar.sync 1, 256;" ::: "memory");
     if (tid < 32) {         // the blocks' sums, to those before each
-        double v = lane < (n + 31) / 32 ? s.before[lane] : 0.0;
-        const double own = v;
+        double v = lane < HT_BLOCKS ? s.before[lane] : 0.0;
 #pragma unroll
         for (int o = 1; o < HT_BLOCKS; o <<= 1) {
             const double a = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += a;
         }
+        const double before = __shfl_up_sync(0xffffffffu, v, 1);
         if (lane <= HT_BLOCKS) {
-            s.before[lane] = v - own;
-            reinterpret_cast<double*>(record + 2 * p.seg)[lane] = v - own;
+            s.before[lane] = lane ? before : 0.0;
+            reinterpret_cast<double*>(record + 2 * p.seg)[lane] = lane ? before : 0.0;
         }
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    asm volatile("bar.sync 1, 256;" ::: "memory");
 }
 
 // ---- U of a segment -----------------------------------------------------------------------------------------------------
@@ -141,21 +142,20 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 7);
     const int warp = warp_number(), lane = threadIdx.x & 31;
     const int h = p.h0 + blockIdx.y;
-    const HdSegment s = hd_find(p, blockIdx.x);
-    if (s.b < 0) return;
+    const uint32_t bar0 = smem_u32(bars), full = bar0, ready = bar0 + 8, empty = bar0 + 16;
     if (sk & 1023u) {
         if (threadIdx.x == 0) atomicCAS(a.error, 0, 49);
         return;
     }
-    const int tiles = (s.n + HT_TILE - 1) / HT_TILE, kv = h / (p.H / p.G);
-    const uint32_t bar0 = smem_u32(bars), full = bar0, ready = bar0 + 8, empty = bar0 + 16;
     if (threadIdx.x == 0) {
         mbar_init(full, 1);
-        mbar_init(ready, 4);
+        mbar_init(ready, HT_WORKERS / 32);
         mbar_init(empty, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
+    const HdSegment s = hd_find(p, blockIdx.x);
+    const int tiles = (s.n + HT_TILE - 1) / HT_TILE, kv = h / (p.H / p.G);      // no tiles: no such segment
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -192,8 +192,8 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             }
             __syncwarp();
         }
-    } else {
-        const int tid = threadIdx.x - 64, quad = warp & 3;
+    } else if (tiles > 0) {
+        const int tid = threadIdx.x - 64, quad = warp & 3, half = tid >> 7, key = tid & 127;
         const size_t at = (size_t)blockIdx.y * p.max_segs + blockIdx.x;
         ht_sums(p, h, s.t0, s.n, tid, sums, a.sums + at * ht_record(p.seg));
         const int blocks = (s.n + 31) / 32;
@@ -202,17 +202,17 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         for (int j = 0; j < tiles && ok; ++j) {
             ok = mbar_wait_warp(full, j & 1, a.error, 43);
             if (!ok) break;
-            const int token = j * HT_TILE + tid;
+            const int token = j * HT_TILE + key;
             const bool there = token < s.n;
             const float w = there ? expf(sums.e[token] + (float)(end - sums.before[(token >> 5) + 1])) : 0.f;
             F2 w2;
             w2.f = make_float2(w, w);
-            uint8_t* row = smem_raw + tid * 128;
+            // two threads a key, every other pair of 16-byte pieces each
 #pragma unroll 1
             for (int b = 0; b < KB; ++b)
-#pragma unroll 4
-                for (int i = 0; i < 8; ++i) {
-                    uint4* at = reinterpret_cast<uint4*>(row + b * BOX + ((i ^ (tid & 7)) << 4));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint4* at = reinterpret_cast<uint4*>(smem_raw + key * 128 + b * BOX + (((half * 4 + i) ^ (key & 7)) << 4));
                     const uint4 x = there ? *at : make_uint4(0u, 0u, 0u, 0u);
                     const uint32_t in[4] = {x.x, x.y, x.z, x.w};
                     uint32_t hi[4], lo[4];
@@ -231,11 +231,11 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(at) + K_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             if (!there) {           // another sequence's values: 0 times one that is no number would not be 0
-                uint8_t* vr = smem_raw + 2 * K_BYTES + tid * 128;
+                uint8_t* vr = smem_raw + 2 * K_BYTES + key * 128 + half * 64;
 #pragma unroll
                 for (int b = 0; b < VB; ++b)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(vr + b * BOX + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(vr + b * BOX + i * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -244,13 +244,13 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         if (ok) ok = mbar_wait_warp(empty, (tiles - 1) & 1, a.error, 44);
         tc_fence_after();
         if (ok) {
-            // accumulators of 64 rows lie in the first 16 lanes of each warp's 32.  A row goes through shared memory (free by now) and leaves
-            // as one bulk copy; rows 16 bytes more than their entries apart, so that lanes do not meet in the banks
-            const int r = DK == 128 ? quad * 32 + lane : quad * 16 + lane;
+            // accumulators of 64 rows lie in the first 16 lanes of each warp's 32.  Half a row goes through shared memory (free by now) and
+            // leaves as one bulk copy; rows 16 bytes more than their entries apart, so that lanes do not meet in the banks
+            const int r = DK == 128 ? quad * 32 + lane : quad * 16 + lane, c_lo = half * (DV / 2);
             const bool mine = r < p.dim && (DK == 128 || lane < 16);
             uint8_t* stage = smem_raw + r * (DV * 4 + 16);
 #pragma unroll 1
-            for (int c0 = 0; c0 < DV; c0 += 32) {
+            for (int c0 = c_lo; c0 < c_lo + DV / 2; c0 += 32) {
                 float o[32];
                 tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + c0, o);
                 if (mine) {
@@ -259,10 +259,10 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         *reinterpret_cast<float4*>(stage + (c0 + i) * 4) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 }
             }
-            if (mine) {
+            if (mine && c_lo < p.vdim) {
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.work + (at * p.dim + r) * p.vdim),
-                             "r"(smem_u32(stage)), "r"(p.vdim * 4) : "memory");
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.work + (at * p.dim + r) * p.vdim + c_lo),
+                             "r"(smem_u32(stage + c_lo * 4)), "r"(min(p.vdim - c_lo, DV / 2) * 4) : "memory");
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
             }
@@ -315,54 +315,52 @@ __global__ void __launch_bounds__(256) hd_pass_tc_kernel(const HdTcArgs a) {
 // ---- outputs -------------------------------------------------------------------------------------------------------------------
 // A weight of 0 times a value that is no number would reach the rows before it: in the 128 keys that a block's rows share such values
 // are made 0 for the product (and the rows of other sequences all of them), and the rows that do see them become NaN at the end.
-// One thread a key.
+// Two threads a key, half of each box's 64 entries.
 template <int VB>
-__device__ __forceinline__ void ht_clear(uint8_t* v, int key, bool there, volatile uint32_t* found) {
+__device__ __forceinline__ void ht_clear(uint8_t* v, int key, int half, bool there, volatile uint32_t* found) {
     uint8_t* row = v + key * 128;
-    const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
     if (!there) {
 #pragma unroll
-        for (int i = 0; i < VB * 8; ++i) *reinterpret_cast<uint4*>(row + (i >> 3) * (HT_TILE * 128) + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < VB * 4; ++i) *reinterpret_cast<uint4*>(row + (i >> 2) * (HT_TILE * 128) + half * 64 + (i & 3) * 16) = make_uint4(0u, 0u, 0u, 0u);
         return;
     }
-    {
-        __nv_bfloat162 sum[4] = {zero, zero, zero, zero};     // of 0 times the entries: 0, or NaN
+    const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
+    __nv_bfloat162 sum[4] = {zero, zero, zero, zero};     // of 0 times the entries: 0, or NaN
 #pragma unroll
-        for (int b = 0; b < VB; ++b)
+    for (int b = 0; b < VB; ++b)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint4 x = *reinterpret_cast<const uint4*>(row + b * (HT_TILE * 128) + ((i ^ (key & 7)) << 4));
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        for (int i = 0; i < 4; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4*>(row + b * (HT_TILE * 128) + (((half * 4 + i) ^ (key & 7)) << 4));
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum[e] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]), zero, sum[e]);
-            }
-        sum[0] = __hadd2(__hadd2(sum[0], sum[1]), __hadd2(sum[2], sum[3]));
-        if ((*reinterpret_cast<const uint32_t*>(&sum[0]) & 0x7fff7fffu) == 0) return;
-        *found = 1;
-    }
-    for (int i = 0; i < VB * 32; ++i) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(row + (i >> 5) * (HT_TILE * 128)) + (i & 31);
+            for (int e = 0; e < 4; ++e) sum[e] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]), zero, sum[e]);
+        }
+    sum[0] = __hadd2(__hadd2(sum[0], sum[1]), __hadd2(sum[2], sum[3]));
+    if ((*reinterpret_cast<const uint32_t*>(&sum[0]) & 0x7fff7fffu) == 0) return;
+    *found = 1;
+    for (int i = 0; i < VB * 16; ++i) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(row + (i >> 4) * (HT_TILE * 128) + (((half * 4 + ((i >> 2) & 3)) ^ (key & 7)) << 4)) + (i & 3);
         *w = finite_pair(*w);
     }
 }
 
 // The row's outputs in the channels where one of the block's tokens up to its own has a value that is no number (gated: all of them, through
 // the norm); `seen`: the block's values.
-__device__ __noinline__ void ht_unclear(const __nv_bfloat16* seen, long long ldv, int vdim, int row, bool all, uint8_t* mine) {
+__device__ __noinline__ void ht_unclear(const __nv_bfloat16* seen, long long ldv, int vdim, int c_lo, int c_hi, int row, bool all, uint8_t* mine) {
     bool any = false;
     for (int pass = 0; pass < (all ? 2 : 1); ++pass)
         for (int c = 0; c < vdim; ++c) {
             bool bad = pass == 1 && any;
             for (int k = 0; k <= row && !bad; ++k) bad = !(fabsf(__bfloat162float(seen[(size_t)k * ldv + c])) < INFINITY);
             any = any || bad;
-            if (bad)
+            if (bad && c >= c_lo && c < c_hi)
                 *reinterpret_cast<uint16_t*>(mine + (c >> 6) * (HT_TILE * 128) + ((((c & 63) >> 3) ^ (row & 7)) << 4) + (c & 7) * 2) = 0x7fff;
         }
 }
 
 struct alignas(16) HtRowsShared {
     float e[HT_MOST * HT_TILE], by_key[HT_MOST * HT_TILE];       // e_j and e^{e_j}
-    float norm[256];
+    float norm[256], squares[2][HT_TILE];
     double before[HT_BLOCKS + 2];
 };
 
@@ -384,16 +382,13 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 11);
     volatile uint32_t* cleared = &tmem_slot + 1;
     const int warp = warp_number(), lane = threadIdx.x & 31;
-    const int h = p.h0 + blockIdx.y, x = blockIdx.x / a.tiles, last = blockIdx.x - x * a.tiles;     // this block's tile of its segment
-    const HdSegment s = hd_find(p, x);
-    if (s.b < 0 || last * HT_TILE >= s.n) return;
+    const int h = p.h0 + blockIdx.y, x = blockIdx.x / a.tiles;
+    const uint32_t bar0 = smem_u32(bars), q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 16, v_full = bar0 + 24, v_empty = bar0 + 32,
+                   s_full = bar0 + 40, p_ready = bar0 + 48, o_start = bar0 + 56, o_done = bar0 + 64, g_full = bar0 + 72;
     if (sq & 1023u) {
         if (threadIdx.x == 0) atomicCAS(a.error, 0, 49);
         return;
     }
-    const int q0 = s.t0 + last * HT_TILE, nq = min(HT_TILE, s.n - last * HT_TILE), kv = h / (p.H / p.G);
-    const uint32_t bar0 = smem_u32(bars), q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 16, v_full = bar0 + 24, v_empty = bar0 + 32,
-                   s_full = bar0 + 40, p_ready = bar0 + 48, o_start = bar0 + 56, o_done = bar0 + 64, g_full = bar0 + 72;
     if (threadIdx.x == 0) {
         *cleared = 0;
         mbar_init(q_full, 1);
@@ -402,18 +397,22 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         mbar_init(v_full, 1);
         mbar_init(v_empty, 1);
         mbar_init(s_full, 1);
-        mbar_init(p_ready, 4);
+        mbar_init(p_ready, HT_WORKERS / 32);
         mbar_init(o_start, 1);
         mbar_init(o_done, 1);
         mbar_init(g_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
+    const HdSegment s = hd_find(p, x);
+    const int last = blockIdx.x - x * a.tiles;              // this block's tile of its segment
+    const int q0 = s.t0 + last * HT_TILE, nq = min(HT_TILE, s.n - last * HT_TILE), kv = h / (p.H / p.G);     // nq <= 0: no such tile
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_o = tmem_slot, tmem_s = tmem_slot + DV;
-    if (warp == 0) {
+    if (nq <= 0) {
+    } else if (warp == 0) {
         // what v's place holds first is S_0
         if (elect_one()) {
             mbar_expect_tx(q_full, K_BYTES);
@@ -501,7 +500,9 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             tc_fence_after();
             if (elect_one()) {
                 const int steps = j < last ? HT_TILE / 16 : (nq + 15) / 16;
-                for (int k = 0; k < steps; ++k) umma_bf16_ts(tmem_o, tmem_s + 8 * k, ht_desc(sv + k * 2048, BOX), idesc_o, 1);
+                // 16 keys are 8 columns of packed pairs; the second 64 keys' lie where their own scores began
+                for (int k = 0; k < steps; ++k)
+                    umma_bf16_ts(tmem_o, tmem_s + 8 * k + (k < 4 ? 0 : 32), ht_desc(sv + k * 2048, BOX), idesc_o, 1);
                 umma_commit(v_empty);
                 umma_commit(o_done);
             }
@@ -514,28 +515,35 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             }
         }
     } else {
-        const int tid = threadIdx.x - 64, quad = warp & 3, row = quad * 32 + lane;
+        const int tid = threadIdx.x - 64, quad = warp & 3, half = tid >> 7, row = quad * 32 + lane, c_lo = half * (DV / 2);
         const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
-        const float* record = a.sums + ((size_t)blockIdx.y * p.max_segs + x) * ht_record(p.seg);
         const bool in = row < nq;
-        const int block = last * 4 + quad;
-        const float e_row = record[last * HT_TILE + row] * HT_LOG2E, l_row = record[p.seg + last * HT_TILE + row];
-        for (int u = tid; u < (last + 1) * HT_TILE; u += HT_TILE) {
-            const float e = record[u];
-            sh.e[u] = e;
-            sh.by_key[u] = ht_ex2(e * HT_LOG2E);
+        // everything that comes from memory is asked for before any of it is used
+        constexpr int U = HT_MOST * HT_TILE / HT_WORKERS;
+        const float* __restrict__ record = a.sums + ((size_t)blockIdx.y * p.max_segs + x) * ht_record(p.seg);
+        const int n_keys = (last + 1) * HT_TILE, mine_at = last * HT_TILE + row;
+        float e[U], norm = 0.f;
+        double before = 0.0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) e[u] = tid + HT_WORKERS * u < n_keys ? record[tid + HT_WORKERS * u] : 0.f;
+        const float l_row = record[p.seg + mine_at], e_row = record[mine_at] * HT_LOG2E;
+        if (tid <= HT_BLOCKS) before = reinterpret_cast<const double*>(record + 2 * p.seg)[tid];
+        if (p.gate && tid < p.vdim) norm = p.norm[(size_t)h * p.vdim + tid];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            sh.e[tid + HT_WORKERS * u] = e[u];
+            sh.by_key[tid + HT_WORKERS * u] = ht_ex2(e[u] * HT_LOG2E);
         }
-        if (tid <= HT_BLOCKS) sh.before[tid] = reinterpret_cast<const double*>(record + 2 * p.seg)[tid];
-        if (p.gate)
-            for (int c = tid; c < p.vdim; c += HT_TILE) sh.norm[c] = p.norm[(size_t)h * p.vdim + c];
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        const double at_block = sh.before[block];
+        if (tid <= HT_BLOCKS) sh.before[tid] = before;
+        sh.norm[tid] = norm;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const double at_block = sh.before[last * 4 + quad];
         bool ok = mbar_wait_warp(o_start, 0, a.error, 47);
         tc_fence_after();
         if (ok) {
             const float f = ht_ex2((l_row + (float)at_block) * HT_LOG2E);
 #pragma unroll 1
-            for (int c0 = 0; c0 < DV; c0 += 32) {
+            for (int c0 = c_lo; c0 < c_lo + DV / 2; c0 += 32) {
                 float o[32];
                 tmem_ld32(tmem_o + lane_sel + c0, o);
 #pragma unroll
@@ -548,7 +556,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             tc_fence_after();
             if (!ok) break;
 #pragma unroll 1
-            for (int b = 0; b < 4; ++b) {
+            for (int b = 2 * half; b < 2 * half + 2; ++b) {
                 uint32_t w[16];
                 float v[32];
                 if (j < last || b <= quad) tmem_ld32(tmem_s + lane_sel + 32 * b, v);
@@ -588,12 +596,12 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 #pragma unroll
                     for (int i = 0; i < 16; ++i) w[i] = 0u;
                 }
-                ht_store16(tmem_s + lane_sel + 16 * b, w);
+                ht_store16(tmem_s + lane_sel + 16 * b + 32 * half, w);      // over scores that this warp has read
             }
             if (j == last) {
                 ok = mbar_wait_warp(v_full, (j + 1) & 1, a.error, 47);
                 if (!ok) break;
-                ht_clear<VB>(smem_raw + QK_BYTES, tid, tid < nq, cleared);
+                ht_clear<VB>(smem_raw + QK_BYTES, tid & 127, half, (tid & 127) < nq, cleared);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -603,25 +611,29 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         if (ok) ok = mbar_wait_warp(o_done, last & 1, a.error, 48);
         tc_fence_after();
-        asm volatile("bar.sync 1, 128;" ::: "memory");          // *cleared, as any of the four warps left it
+        asm volatile("bar.sync 1, 256;" ::: "memory");          // *cleared, as any of the four warps left it
         if (ok && p.gate) ok = mbar_wait_warp(g_full, 0, a.error, 48);
-        if (ok) {
-            float by = p.scale;
-            if (p.gate) {
+        float by = p.scale;
+        if (p.gate) {
+            if (ok) {
                 float sq2 = 0.f;
 #pragma unroll 1
-                for (int c0 = 0; c0 < DV; c0 += 32) {
+                for (int c0 = c_lo; c0 < c_lo + DV / 2; c0 += 32) {
                     float o[32];
                     tmem_ld32(tmem_o + lane_sel + c0, o);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) sq2 += o[i] * o[i];
                 }
-                by *= rsqrtf(sq2 * (p.scale * p.scale) / (float)p.vdim + p.eps);
+                sh.squares[half][row] = sq2;
             }
+            asm volatile("bar.sync 2, 256;" ::: "memory");
+            by *= rsqrtf((sh.squares[0][row] + sh.squares[1][row]) * (p.scale * p.scale) / (float)p.vdim + p.eps);
+        }
+        if (ok) {
             // the row's outputs go where its gate is (16-byte pieces in the order of the TMA's swizzle) ...
             uint8_t* mine = smem_raw + row * 128;
 #pragma unroll 1
-            for (int c0 = 0; c0 < DV; c0 += 32) {
+            for (int c0 = c_lo; c0 < c_lo + DV / 2; c0 += 32) {
                 float o[32];
                 tmem_ld32(tmem_o + lane_sel + c0, o);
 #pragma unroll
@@ -642,16 +654,17 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                 }
             }
             if (*cleared && in)
-                ht_unclear(static_cast<const __nv_bfloat16*>(p.v) + (size_t)q0 * p.ldv + (size_t)kv * p.vdim, p.ldv, p.vdim, row, p.gate != nullptr, mine);
+                ht_unclear(static_cast<const __nv_bfloat16*>(p.v) + (size_t)q0 * p.ldv + (size_t)kv * p.vdim, p.ldv, p.vdim, c_lo, min(p.vdim, c_lo + DV / 2), row,
+                           p.gate != nullptr, mine);
             __syncwarp();
             // ... and leave in whole lines, the warp's rows one after the other
-            const int pieces = p.vdim >> 3, rows = min(32, nq - quad * 32);
-            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (size_t)(q0 + quad * 32) * p.ldo + (size_t)h * p.vdim;
+            const int pieces = (min(p.vdim, c_lo + DV / 2) - c_lo) >> 3, rows = min(32, nq - quad * 32);
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + (size_t)(q0 + quad * 32) * p.ldo + (size_t)h * p.vdim + c_lo;
 #pragma unroll 4
             for (int i = lane; i < rows * pieces; i += 32) {
-                const int r = i / pieces, c = i - r * pieces, rr = quad * 32 + r;
+                const int r = i / pieces, at = i - r * pieces, c = c_lo / 8 + at, rr = quad * 32 + r;
                 const uint4 y = *reinterpret_cast<const uint4*>(smem_raw + rr * 128 + (c >> 3) * BOX + (((c & 7) ^ (rr & 7)) << 4));
-                *reinterpret_cast<uint4*>(dst + (size_t)r * p.ldo + c * 8) = y;
+                *reinterpret_cast<uint4*>(dst + (size_t)r * p.ldo + at * 8) = y;
             }
         }
     }

@@ -15,7 +15,7 @@
 #include "common.cuh"
 
 #define RG_MAX_E 1024
-#define RG_MAX_K 31
+#define RG_MAX_K 30
 #define RG_MAX_GROUPS 32
 #define RG_WARPS 8
 
@@ -38,39 +38,70 @@ __device__ __forceinline__ float rg_value(unsigned key) {
     return key == 1u ? __int_as_float(0x7fc00000) : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// c of expert e in 64 bits; NaN as below every number.
-__device__ __forceinline__ double rg_rank64(const RouterGroupArgs& p, float x, int e, float mx, double inv) {
-    const double s = p.softmax ? exp((double)x - (double)mx) * inv : 1.0 / (1.0 + exp(-(double)x));
-    return s + (p.bias ? (double)p.bias[e] : 0.0);
+// Entries e0 .. e0 + PER - 1 of a row of E, `none` behind its end; four an access where they lie so.
+template <int PER>
+__device__ __forceinline__ void rg_load(const float* __restrict__ row, int e0, int E, float none, float (&x)[PER]) {
+    if constexpr (PER >= 4) {
+        if (((uintptr_t)row & 15) == 0 && e0 + PER <= E) {
+#pragma unroll
+            for (int i = 0; i < PER; i += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(row + e0 + i);
+                x[i] = f.x;
+                x[i + 1] = f.y;
+                x[i + 2] = f.z;
+                x[i + 3] = f.w;
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = e0 + i < E ? row[e0 + i] : none;
 }
 
-// The choice in 64 bits, by plain steps: called for the few rows where float cannot tell.  Returns this lane's choice (lane < k).
+// The choice in 64 bits: called for the few rows where float cannot tell.  Returns this lane's choice (lane < k).
 template <int PER>
 __device__ __noinline__ int rg_choose64(const RouterGroupArgs& p, const float* row, float mx, int lane) {
     const double lowest = -INFINITY;
-    double c[PER], sum = 0.0;
-    bool open[PER];                 // may be chosen
+    const int size = p.E / p.groups;
+    double c[PER];
+    unsigned open = 0u;             // which of the lane's may be chosen
+#pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int e = lane * PER + i;
-        open[i] = e < p.E;
-        if (open[i] && p.softmax) sum += exp((double)row[e] - (double)mx);
+        const float x = e < p.E ? row[e] : -INFINITY;
+        c[i] = p.softmax ? exp((double)x - (double)mx) : 1.0 / (1.0 + exp(-(double)x));
+        if (e < p.E) open |= 1u << i;
     }
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const double inv = sum > 0.0 ? 1.0 / sum : sum == 0.0 ? 0.0 : sum;
-    for (int i = 0; i < PER; ++i) c[i] = open[i] ? rg_rank64(p, row[lane * PER + i], lane * PER + i, mx, inv) : lowest;
+    if (p.softmax) {
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) sum += c[i];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const double inv = sum == 0.0 ? 0.0 : 1.0 / sum;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) c[i] *= inv;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (p.bias && (open >> i & 1u)) c[i] += (double)p.bias[lane * PER + i];
+        if (c[i] != c[i]) c[i] = lowest;
+    }
     if (p.groups > 1) {
-        const int size = p.E / p.groups;
         double worth = lowest;      // of group `lane`
         for (int g = 0; g < p.groups; ++g) {
-            double a = lowest, b = lowest;      // the two largest
+            const int from = g * size - lane * PER;         // the group among this lane's
+            double a = lowest, b = lowest;      // its two largest
+#pragma unroll
             for (int i = 0; i < PER; ++i)
-                if (open[i] && (lane * PER + i) / size == g) {
-                    if (c[i] > a) { b = a; a = c[i]; }
-                    else if (c[i] > b) b = c[i];
+                if (i >= from && i < from + size) {
+                    b = fmax(b, fmin(a, c[i]));
+                    a = fmax(a, c[i]);
                 }
+#pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
                 const double oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
-                b = oa > a ? fmax(a, ob) : fmax(b, oa);
+                b = fmax(fmin(a, oa), fmax(b, ob));
                 a = fmax(a, oa);
             }
             if (lane == g) worth = p.group_top == 2 && size > 1 ? a + b : a;
@@ -81,19 +112,25 @@ __device__ __noinline__ int rg_choose64(const RouterGroupArgs& p, const float* r
             place += other > worth || (other == worth && g < lane);
         }
         const unsigned kept = __ballot_sync(0xffffffffu, lane < p.groups && place < p.groups_use);
-        for (int i = 0; i < PER; ++i) open[i] = open[i] && (kept >> ((lane * PER + i) / size) & 1u);
+        for (int g = 0; g < p.groups; ++g) {
+            const int from = g * size - lane * PER;
+            if (kept >> g & 1u) continue;
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (i >= from && i < from + size) open &= ~(1u << i);
+        }
     }
     int mine = 0;
     for (int j = 0; j < p.k; ++j) {
         double best = lowest;
         int at = 0x7fffffff;
-        for (int i = 0; i < PER; ++i) {
-            const double v = c[i] != c[i] ? lowest : c[i];
-            if (open[i] && (at == 0x7fffffff || v > best)) {
-                best = v;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if ((open >> i & 1u) && (at == 0x7fffffff || c[i] > best)) {
+                best = c[i];
                 at = lane * PER + i;
             }
-        }
+#pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const double ov = __shfl_xor_sync(0xffffffffu, best, o);
             const int oi = __shfl_xor_sync(0xffffffffu, at, o);
@@ -102,8 +139,7 @@ __device__ __noinline__ int rg_choose64(const RouterGroupArgs& p, const float* r
                 at = oi;
             }
         }
-        for (int i = 0; i < PER; ++i)
-            if (lane * PER + i == at) open[i] = false;
+        if (at / PER == lane) open &= ~(1u << (at - lane * PER));
         if (lane == j) mine = at;
     }
     return mine;
@@ -119,26 +155,7 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_groups_kernel(const Rout
     const float* row = p.logits + t * p.ld;
     const int E = p.E, e0 = lane * PER;
     float x[PER];
-    if (PER >= 4 && (((uintptr_t)row & 15) == 0)) {
-#pragma unroll
-        for (int i = 0; i < PER; i += 4) {
-            if (e0 + i + 4 <= E) {
-                const float4 f = *reinterpret_cast<const float4*>(row + e0 + i);
-                x[i] = f.x;
-                if (PER >= 4) {
-                    x[(i + 1) % PER] = f.y;
-                    x[(i + 2) % PER] = f.z;
-                    x[(i + 3) % PER] = f.w;
-                }
-            } else {
-#pragma unroll
-                for (int l = 0; l < 4; ++l) x[(i + l) % PER] = e0 + i + l < E ? row[e0 + i + l] : -INFINITY;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) x[i] = e0 + i < E ? row[e0 + i] : -INFINITY;
-    }
+    rg_load<PER>(row, e0, E, -INFINITY, x);
     // scores, as far as they are asked for
     const bool sums = p.groups > 1 && p.group_top == 2;     // sums of scores decide
     const bool by_logit = !p.bias;
@@ -158,12 +175,30 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_groups_kernel(const Rout
     auto score = [&](float v) { return p.softmax ? expf(v - mx) * inv : 1.0f / (1.0f + expf(-v)); };
     unsigned key[PER];
     float c[PER];
+    if (by_logit && !sums) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        c[i] = by_logit && !sums ? x[i] : score(x[i]);
-        if (p.bias && e0 + i < E) c[i] += p.bias[e0 + i];
-        key[i] = e0 + i < E ? rg_key(by_logit ? x[i] : c[i]) : 0u;
+        for (int i = 0; i < PER; ++i) c[i] = x[i];
+    } else {
+        // the hardware's exponential and reciprocal (2 and 1 ulp, and the argument's rounding): off by 3e-7 of the largest score at most,
+        // within what `loose` below allows for
+        const float by = p.softmax ? 1.4426950408889634f : -1.4426950408889634f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            float y;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((x[i] - mx) * by));
+            if (p.softmax) y *= inv;
+            else asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + y));
+            c[i] = y;
+        }
+        if (p.bias) {
+            float b[PER];
+            rg_load<PER>(p.bias, e0, E, 0.f, b);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) c[i] += b[i];
+        }
     }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) key[i] = e0 + i < E ? rg_key(by_logit ? x[i] : c[i]) : 0u;
     // what float may have turned round: scores up to `top`, each off by up to 4 (sigmoid) or 24 (softmax, its sum included)
     // half steps of it, and the roundings of the sums that were compared
     const float loose = (p.softmax ? 24.f * inv : 4.f) * 1.2e-7f;
@@ -176,6 +211,7 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_groups_kernel(const Rout
             if (e0 + i < E) cs[e0 + i + ((e0 + i) >> 5)] = c[i] != c[i] ? -INFINITY : c[i];
         __syncwarp();
         const int size = E / p.groups;
+        const float per_size = 1.0f / (float)size;      // (e + 1/2) / size is at least 1 / 2048 from a whole number
         int L = 1;
         while (2 * L * p.groups <= 32) L *= 2;
         const int g = lane / L, part = lane - g * L;
@@ -211,44 +247,104 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_groups_kernel(const Rout
         const unsigned kept = __ballot_sync(0xffffffffu, in);
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            if (e0 + i < E && !(kept >> ((e0 + i) / size * L) & 1u)) key[i] = 0u;
+            if (!(kept >> ((int)((e0 + i + 0.5f) * per_size) * L & 31) & 1u)) key[i] = 0u;
     }
-    // the k largest, and the one that would come next
-    unsigned most = key[0], my_key = 0u;
-#pragma unroll
-    for (int i = 1; i < PER; ++i) most = max(most, key[i]);
+    // the k largest, and where float may have turned values round the two that would come next
+    unsigned my_key = 0u;
     int mine = 0;
-    for (int j = 0; j <= p.k; ++j) {
-        const unsigned best = __reduce_max_sync(0xffffffffu, most);
-        const int from = __ffs(__ballot_sync(0xffffffffu, most == best)) - 1;
-        int at = 0;
-        if (lane == from) {
-            bool found = false;
+    const int rounds = by_logit ? p.k : p.k + 2;
+    if constexpr (PER <= 8) {
+        // a lane's own in descending order first (neighbours change places only if the later is larger, so equals stay in order), their
+        // places in four bits each: the lane that a round takes from moves up
+        unsigned place[PER], places = 0u;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) place[i] = i;
+#pragma unroll
+        for (int turn = 0; turn < PER; ++turn)
+#pragma unroll
+            for (int i = turn & 1; i + 1 < PER; i += 2) {
+                const bool swap = key[i + 1] > key[i];
+                const unsigned k0 = key[i], p0 = place[i];
+                key[i] = swap ? key[i + 1] : k0;
+                key[i + 1] = swap ? k0 : key[i + 1];
+                place[i] = swap ? place[i + 1] : p0;
+                place[i + 1] = swap ? p0 : place[i + 1];
+            }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) places |= place[i] << (4 * i);
+        for (int j = 0; j < rounds; ++j) {
+            const unsigned best = __reduce_max_sync(0xffffffffu, key[0]);
+            const int from = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
+            const int e = __shfl_sync(0xffffffffu, e0 + (int)(places & 15u), from);
+            const bool taken = lane == from;
+#pragma unroll
+            for (int i = 0; i + 1 < PER; ++i) key[i] = taken ? key[i + 1] : key[i];
+            key[PER - 1] = taken ? 0u : key[PER - 1];
+            places = taken ? places >> 4 : places;
+            if (lane == j) {
+                my_key = best;
+                mine = e;
+            }
+        }
+    } else {
+        unsigned most = key[0];
+#pragma unroll
+        for (int i = 1; i < PER; ++i) most = max(most, key[i]);
+        for (int j = 0; j < rounds; ++j) {
+            const unsigned best = __reduce_max_sync(0xffffffffu, most);
+            const int from = __ffs(__ballot_sync(0xffffffffu, most == best)) - 1;
+            int at = PER;
+#pragma unroll
+            for (int i = PER - 1; i >= 0; --i) at = key[i] == best ? i : at;
+            const int e = __shfl_sync(0xffffffffu, e0 + at, from);
+            if (lane != from) at = PER;
             most = 0u;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                if (!found && key[i] == best) {
-                    found = true;
-                    at = e0 + i;
-                    key[i] = 0u;
-                }
+                key[i] = i == at ? 0u : key[i];
                 most = max(most, key[i]);
             }
-        }
-        at = __shfl_sync(0xffffffffu, at, from);
-        if (lane == j) {
-            my_key = best;
-            mine = at;
+            if (lane == j) {
+                my_key = best;
+                mine = e;
+            }
         }
     }
-    float mine_x = lane <= p.k && my_key ? row[mine] : 0.f;
+    const bool have = lane < rounds && my_key != 0u;        // fewer than k + 2 may be left
+    if (!have) mine = 0;
+    float mine_x = have ? row[mine] : 0.f;
     if (!by_logit) {
-        const float v = rg_value(my_key), nv = __shfl_down_sync(0xffffffffu, v, 1), nx = __shfl_down_sync(0xffffffffu, mine_x, 1);
-        const unsigned nk = __shfl_down_sync(0xffffffffu, my_key, 1);
-        const float mb = lane <= p.k && my_key ? p.bias[mine] : 0.f, nb = __shfl_down_sync(0xffffffffu, mb, 1);
-        const bool close = lane < p.k && my_key && nk && v - nv <= 2.f * loose + 1.3e-7f * (fabsf(v) + fabsf(nv)) &&
-                           !(mine_x == nx && mb == nb);
-        again = again || close;
+        // a lane's value against its follower's
+        const float v = rg_value(my_key), b = have ? p.bias[mine] : 0.f, nv = __shfl_down_sync(0xffffffffu, v, 1);
+        const float nx = __shfl_down_sync(0xffffffffu, mine_x, 1), nb = __shfl_down_sync(0xffffffffu, b, 1);
+        const bool followed = __shfl_down_sync(0xffffffffu, (int)have, 1) && have && lane + 1 < rounds;
+        const bool near = followed && v - nv <= 2.f * loose + 1.3e-7f * (fabsf(v) + fabsf(nv));
+        const unsigned nears = __ballot_sync(0xffffffffu, near);
+        const unsigned closes = __ballot_sync(0xffffffffu, near && !(mine_x == nx && b == nb));
+        if (!again) {
+            if ((nears >> (p.k - 1) & 3u) == 3u) {
+                again = true;       // one that was not looked at may belong among the chosen
+            } else if ((closes & ((1u << p.k) - 1u)) && p.softmax) {
+                again = true;       // a sum over all experts is wanted
+            } else if (closes & ((1u << p.k) - 1u)) {
+                // the candidates in 64 bits, a lane each, to their places by counting
+                const double d = have && lane <= p.k ? 1.0 / (1.0 + exp(-(double)mine_x)) + (double)b : 0.0;
+                const bool counts = have && lane <= p.k;
+                int place = 0;
+                for (int j = 0; j <= p.k; ++j) {
+                    const double od = __shfl_sync(0xffffffffu, d, j);
+                    const int oe = __shfl_sync(0xffffffffu, mine, j);
+                    const int there = __shfl_sync(0xffffffffu, (int)counts, j);
+                    place += there && (od > d || (od == d && oe < mine));
+                }
+                const int was = mine;
+                for (int j = 0; j <= p.k; ++j) {
+                    const int to = __shfl_sync(0xffffffffu, counts ? place : 32, j), e = __shfl_sync(0xffffffffu, was, j);
+                    if (lane == to) mine = e;
+                }
+                if (lane < p.k) mine_x = row[mine];
+            }
+        }
     }
     if (__any_sync(0xffffffffu, again)) {
         mine = rg_choose64<PER>(p, row, mx, lane);

@@ -25,18 +25,22 @@ WORK_BYTES = 512 << 20          # the most scratch for the segments' states: of 
 
 def _rows(t, name, nt, heads, dim, dtype):
     """The distance of the rows of ``t`` [nt, heads, dim], whose heads lie one behind the other."""
-    if tuple(t.shape) != (nt, heads, dim) or t.dtype != dtype:
+    if t.shape != (nt, heads, dim) or t.dtype != dtype:
         raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, expected {dtype} {(nt, heads, dim)}")
     s = t.stride()
+    if s[2] == 1 and s[1] == dim and s[0] >= heads * dim:
+        return s[0]
     if (s[2] != 1 and dim > 1) or (s[1] != dim and heads > 1) or (s[0] < heads * dim and nt > 1):
         raise ValueError(f"{name}: a row's heads must lie one behind the other, rows apart, got strides {s}")
     return s[0] if nt > 1 else heads * dim
 
 
 def _states(t, name, H, dim, vdim):
-    if t.dim() != 4 or tuple(t.shape[1:]) != (H, dim, vdim) or t.dtype != torch.float32:
+    if t.dim() != 4 or t.shape[1:] != (H, dim, vdim) or t.dtype != torch.float32:
         raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, expected float32 [slots, {H}, {dim}, {vdim}]")
     s = t.stride()
+    if s[3] == 1 and s[2] == vdim and s[1] == dim * vdim and s[0] >= H * s[1]:
+        return s[0]
     if t.numel() and ((s[3] != 1 and vdim > 1) or (s[2] != vdim and dim > 1) or (s[1] != dim * vdim and H > 1) or
                       (s[0] < H * dim * vdim and t.shape[0] > 1)):
         raise ValueError(f"{name}: a slot's state must be contiguous, slots apart, got strides {s}")
@@ -58,7 +62,7 @@ def _checked(q, k, v, log_decay, state, slots, out, norm, gate, new_state):
         raise ValueError(f"heads have 1..{MOST_DIM} entries, got {dim} and {vdim}")
     lds = (_rows(q, "q", nt, H, dim, dtype), _rows(k, "k", nt, G, dim, dtype), _rows(v, "v", nt, G, vdim, dtype))
     ldo = _rows(out, "out", nt, H, vdim, dtype)
-    if log_decay.dtype != torch.float32 or tuple(log_decay.shape) not in ((H,), (nt, H)) or \
+    if log_decay.dtype != torch.float32 or (log_decay.shape != (nt, H) and log_decay.shape != (H,)) or \
             (log_decay.stride(-1) != 1 and H > 1) or (log_decay.dim() == 2 and nt > 1 and log_decay.stride(0) < H):
         raise ValueError(f"log_decay: float32 [{H}] or [{nt}, {H}] with contiguous rows, got {log_decay.dtype} {tuple(log_decay.shape)}")
     g_stride = 0 if log_decay.dim() == 1 else max(log_decay.stride(0), H)

@@ -10,7 +10,7 @@ import torch
 
 from ..csrc import lib
 
-MOST_EXPERTS, MOST_CHOSEN, MOST_GROUPS = 1024, 31, 32       # of the kernel (csrc/router_groups.cu)
+MOST_EXPERTS, MOST_CHOSEN, MOST_GROUPS = 1024, 30, 32       # of the kernel (csrc/router_groups.cu)
 SCORES = ("softmax", "sigmoid")
 
 
@@ -33,7 +33,7 @@ def check_choice(experts: int, k: int, *, scores="softmax", groups=1, groups_use
 def choose_experts(logits, index, weights, *, scores="softmax", bias=None, groups=1, groups_use=1, group_top=1, renorm=False,
                    scale=1.0) -> None:
     """Fill ``index`` (int32) and ``weights`` (float), both [tokens, k] and contiguous, from ``logits``, float [tokens, experts]
-    with contiguous rows, by the formulas at the head of this file; ``bias``: float [experts] or None; up to 31 of 1,024 experts
+    with contiguous rows, by the formulas at the head of this file; ``bias``: float [experts] or None; up to 30 of 1,024 experts
     in up to 32 groups of neighbours.
 
     Equal c, and groups of equal worth, go to the lower index.  A logit of -inf masks an expert: its score is 0, in a row of
@@ -45,10 +45,10 @@ def choose_experts(logits, index, weights, *, scores="softmax", bias=None, group
     check_choice(E, k, scores=scores, groups=groups, groups_use=groups_use, group_top=group_top)
     if logits.dtype != torch.float32 or (logits.stride(1) != 1 and E > 1) or (nt > 1 and logits.stride(0) < E):
         raise ValueError("the choice reads float32 logits with contiguous rows")
-    if tuple(index.shape) != (nt, k) or tuple(weights.shape) != (nt, k) or index.dtype != torch.int32 or \
+    if index.shape != (nt, k) or weights.shape != (nt, k) or index.dtype != torch.int32 or \
             weights.dtype != torch.float32 or not index.is_contiguous() or not weights.is_contiguous():
         raise ValueError(f"index (int32) and weights (float32) must be contiguous [{nt}, {k}] tensors")
-    if bias is not None and (tuple(bias.shape) != (E,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
+    if bias is not None and (bias.shape != (E,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
         raise ValueError(f"the bias must be a contiguous float32 tensor of {E} entries")
     lib.check_device(logits, index, weights, bias)
     lib.call("tb_router_groups", logits.data_ptr(), max(logits.stride(0), E), lib.ptr(bias), index.data_ptr(), weights.data_ptr(),
