@@ -18,6 +18,7 @@
 #include "tc_common.cuh"
 
 #define HT_TILE 128
+#define HT_HALF 64              // rows of a TMA box, and keys that the update takes together
 #define HT_MOST 4               // tiles of a segment
 #define HT_WORKERS 256          // eight warps: two for each 32 lanes of tensor memory, half of the columns each
 #define HT_THREADS (64 + HT_WORKERS)
@@ -46,6 +47,9 @@ __device__ __forceinline__ uint64_t ht_desc(uint32_t smem_addr, uint32_t lbo) { 
     d |= (uint64_t)2 << 61;
     return d;
 }
+__device__ __forceinline__ void ht_fetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 // 16 packed pairs over 16 columns of this thread's lane (tcgen05.wait::st comes before they are handed over)
 __device__ __forceinline__ void ht_store16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
@@ -69,6 +73,15 @@ __device__ __forceinline__ float ht_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// 128 rows of one head from token t on, in boxes of 64 rows and 64 columns, the columns' boxes HT_TILE rows apart
+template <int BOXES>
+__device__ __forceinline__ void ht_load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int head, int t) {
+#pragma unroll
+    for (int b = 0; b < BOXES; ++b)
+#pragma unroll
+        for (int r = 0; r < HT_TILE; r += HT_HALF) tma_load_3d(dst + b * (HT_TILE * 128) + r * 128, map, bar, b * 64, head, t + r);
 }
 
 // The decays of a segment's tokens in blocks of 32: e_j = the sum behind token j to its block's end, l_j = up to and with token j from its
@@ -123,132 +136,146 @@ __device__ __forceinline__ void ht_sums(const HeadDecayArgs& p, int h, int t0, i
 }
 
 // ---- U of a segment -----------------------------------------------------------------------------------------------------
-// Shared memory of the tiles K, what rounding left of K' and V, and of U's rows afterwards.
-__host__ __device__ constexpr int ht_update_area(int kb, int vb) {
-    const int tiles = (2 * kb + vb) * HT_TILE * 128, rows = (kb * 64 * (vb * 256 + 16) + 1023) / 1024 * 1024;
-    return tiles > rows ? tiles : rows;
-}
+// 64 keys at a time in two stages: while one is weighted and multiplied the other is on its way.  U leaves with its entries in the order
+// [vdim / 4][dim][4]: a warp's 32 rows of four columns are 512 bytes on end.
 template <int KB, int VB>
 __global__ void __launch_bounds__(HT_THREADS, VB == 4 ? 1 : 2)
 hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const HdTcArgs a) {
+    if (threadIdx.x == 0) {
+        ht_fetch_map(&map_k);
+        ht_fetch_map(&map_v);
+    }
     pdl_sync();
     constexpr int DK = KB * 64, DV = VB * 64;
-    constexpr uint32_t BOX = HT_TILE * 128, K_BYTES = KB * BOX, V_BYTES = VB * BOX, TMEM_COLS = VB == 4 ? 256 : VB * 64;
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    constexpr uint32_t BOX = HT_HALF * 128, K_BYTES = KB * BOX, V_BYTES = VB * BOX, STAGE = 2 * K_BYTES + V_BYTES, TMEM_COLS = VB == 4 ? 256 : VB * 64;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];       // a stage: K (then K'), what rounding left of K', V
     const HeadDecayArgs& p = a.p;
-    const uint32_t sk = smem_u32(smem_raw), sl = sk + K_BYTES, sv = sl + K_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + ht_update_area(KB, VB));
+    const uint32_t base = smem_u32(smem_raw);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + 2 * STAGE);
     HtSums& sums = *reinterpret_cast<HtSums*>(bars + 8);
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 7);
     const int warp = warp_number(), lane = threadIdx.x & 31;
     const int h = p.h0 + blockIdx.y;
-    const uint32_t bar0 = smem_u32(bars), full = bar0, ready = bar0 + 8, empty = bar0 + 16;
-    if (sk & 1023u) {
+    const uint32_t bar0 = smem_u32(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto ready = [&](int s) { return bar0 + 16 + 8u * s; };
+    auto empty = [&](int s) { return bar0 + 32 + 8u * s; };
+    if (base & 1023u) {
         if (threadIdx.x == 0) atomicCAS(a.error, 0, 49);
         return;
     }
     if (threadIdx.x == 0) {
-        mbar_init(full, 1);
-        mbar_init(ready, HT_WORKERS / 32);
-        mbar_init(empty, 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(ready(s), HT_WORKERS / 32);
+            mbar_init(empty(s), 1);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncwarp();
     if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
     const HdSegment s = hd_find(p, blockIdx.x);
-    const int tiles = (s.n + HT_TILE - 1) / HT_TILE, kv = h / (p.H / p.G);      // no tiles: no such segment
+    const int tiles = (s.n + HT_HALF - 1) / HT_HALF, kv = h / (p.H / p.G);      // no tiles: no such segment
+    auto copy = [&](int j) {
+        if (elect_one()) {
+            const uint32_t sk = base + (j & 1) * STAGE, sv = sk + 2 * K_BYTES;
+            mbar_expect_tx(full(j & 1), K_BYTES + V_BYTES);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) tma_load_3d(sk + b * BOX, &map_k, full(j & 1), b * 64, kv, s.t0 + j * HT_HALF);
+#pragma unroll
+            for (int b = 0; b < VB; ++b) tma_load_3d(sv + b * BOX, &map_v, full(j & 1), b * 64, kv, s.t0 + j * HT_HALF);
+        }
+        __syncwarp();
+    };
+    // the first copies do not wait for the other warps: this one has made their barriers
+    if (warp == 0 && tiles > 0) copy(0);
+    if (warp == 0 && tiles > 1) copy(1);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     if (warp == 0) {
-        int issued = 0;
-        for (int j = 0; j < tiles; ++j) {
-            if (j > 0 && !mbar_wait_warp(empty, (j - 1) & 1, a.error, 41)) break;
-            if (elect_one()) {
-                mbar_expect_tx(full, K_BYTES + V_BYTES);
-#pragma unroll
-                for (int b = 0; b < KB; ++b) tma_load_3d(sk + b * BOX, &map_k, full, b * 64, kv, s.t0 + j * HT_TILE);
-#pragma unroll
-                for (int b = 0; b < VB; ++b) tma_load_3d(sv + b * BOX, &map_v, full, b * 64, kv, s.t0 + j * HT_TILE);
-            }
-            __syncwarp();
+        int issued = min(tiles, 2);
+        for (int j = 2; j < tiles; ++j) {
+            if (!mbar_wait_warp(empty(j & 1), ((j >> 1) - 1) & 1, a.error, 41)) break;
+            copy(j);
             issued = j + 1;
         }
-        if (*(volatile int*)a.error != 0 && issued) mbar_wait(full, (issued - 1) & 1, a.error, 41);
+        if (*(volatile int*)a.error != 0)           // no copy is left under way
+            for (int j = max(0, issued - 2); j < issued; ++j) mbar_wait(full(j & 1), (j >> 1) & 1, a.error, 41);
     } else if (warp == 1) {
         // A = K'^T and B = V, both with the tokens along the rows of their tiles (MN-major)
         const uint32_t idesc = umma_idesc(DK, DV) | (1u << 15) | (1u << 16);
         for (int j = 0; j < tiles; ++j) {
-            if (!mbar_wait_warp(ready, j & 1, a.error, 42)) break;
+            if (!mbar_wait_warp(ready(j & 1), (j >> 1) & 1, a.error, 42)) break;
             tc_fence_after();
             if (elect_one()) {
-                const int steps = (min(HT_TILE, s.n - j * HT_TILE) + 15) / 16;
+                const uint32_t sk = base + (j & 1) * STAGE, sv = sk + 2 * K_BYTES;
+                const int steps = (min(HT_HALF, s.n - j * HT_HALF) + 15) / 16;
                 for (int k = 0; k < steps; ++k) {
                     const uint64_t dv = ht_desc(sv + k * 2048, BOX);
                     umma_bf16(tmem, ht_desc(sk + k * 2048, BOX), dv, idesc, (j | k) != 0);
-                    umma_bf16(tmem, ht_desc(sl + k * 2048, BOX), dv, idesc, 1);
+                    umma_bf16(tmem, ht_desc(sk + K_BYTES + k * 2048, BOX), dv, idesc, 1);
                 }
-                umma_commit(empty);
+                umma_commit(empty(j & 1));
             }
             __syncwarp();
         }
     } else if (tiles > 0) {
-        const int tid = threadIdx.x - 64, quad = warp & 3, half = tid >> 7, key = tid & 127;
+        const int tid = threadIdx.x - 64, quad = warp & 3, key = tid & 63, part = tid >> 6;
         const size_t at = (size_t)blockIdx.y * p.max_segs + blockIdx.x;
         ht_sums(p, h, s.t0, s.n, tid, sums, a.sums + at * ht_record(p.seg));
-        const int blocks = (s.n + 31) / 32;
-        const double end = sums.before[blocks];
+        const double end = sums.before[(s.n + 31) / 32];
         bool ok = true;
         for (int j = 0; j < tiles && ok; ++j) {
-            ok = mbar_wait_warp(full, j & 1, a.error, 43);
+            ok = mbar_wait_warp(full(j & 1), (j >> 1) & 1, a.error, 43);
             if (!ok) break;
-            const int token = j * HT_TILE + key;
+            const int token = j * HT_HALF + key;
             const bool there = token < s.n;
             const float w = there ? expf(sums.e[token] + (float)(end - sums.before[(token >> 5) + 1])) : 0.f;
             F2 w2;
             w2.f = make_float2(w, w);
-            // two threads a key, every other pair of 16-byte pieces each
-#pragma unroll 1
-            for (int b = 0; b < KB; ++b)
+            uint8_t* row = smem_raw + (j & 1) * STAGE + key * 128;
+            // four threads a key, a quarter of its 16-byte pieces each
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint4* at = reinterpret_cast<uint4*>(smem_raw + key * 128 + b * BOX + (((half * 4 + i) ^ (key & 7)) << 4));
-                    const uint4 x = there ? *at : make_uint4(0u, 0u, 0u, 0u);
-                    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-                    uint32_t hi[4], lo[4];
+            for (int i = 0; i < 2 * KB; ++i) {
+                const int piece = part * 2 * KB + i;
+                uint4* at = reinterpret_cast<uint4*>(row + (piece >> 3) * BOX + (((piece & 7) ^ (key & 7)) << 4));
+                const uint4 x = there ? *at : make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+                uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        F2 f, g;
-                        f.f = make_float2(__uint_as_float(in[e] << 16), __uint_as_float(in[e] & 0xffff0000u));
-                        f = mul2(f, w2);
-                        const __nv_bfloat162 r = __floats2bfloat162_rn(f.f.x, f.f.y);
-                        hi[e] = *reinterpret_cast<const uint32_t*>(&r);
-                        g.f = make_float2(f.f.x - __uint_as_float(hi[e] << 16), f.f.y - __uint_as_float(hi[e] & 0xffff0000u));
-                        const __nv_bfloat162 q = __floats2bfloat162_rn(g.f.x, g.f.y);
-                        lo[e] = *reinterpret_cast<const uint32_t*>(&q);
-                    }
-                    *at = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(at) + K_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                for (int e = 0; e < 4; ++e) {
+                    F2 f, g;
+                    f.f = make_float2(__uint_as_float(in[e] << 16), __uint_as_float(in[e] & 0xffff0000u));
+                    f = mul2(f, w2);
+                    const __nv_bfloat162 r = __floats2bfloat162_rn(f.f.x, f.f.y);
+                    hi[e] = *reinterpret_cast<const uint32_t*>(&r);
+                    g.f = make_float2(f.f.x - __uint_as_float(hi[e] << 16), f.f.y - __uint_as_float(hi[e] & 0xffff0000u));
+                    const __nv_bfloat162 q = __floats2bfloat162_rn(g.f.x, g.f.y);
+                    lo[e] = *reinterpret_cast<const uint32_t*>(&q);
                 }
+                *at = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(at) + K_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
             if (!there) {           // another sequence's values: 0 times one that is no number would not be 0
-                uint8_t* vr = smem_raw + 2 * K_BYTES + key * 128 + half * 64;
 #pragma unroll
-                for (int b = 0; b < VB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(vr + b * BOX + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                for (int i = 0; i < 2 * VB; ++i) {
+                    const int piece = part * 2 * VB + i;
+                    *reinterpret_cast<uint4*>(row + 2 * K_BYTES + (piece >> 3) * BOX + (piece & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ready) : "memory");
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ready(j & 1)) : "memory");
         }
-        if (ok) ok = mbar_wait_warp(empty, (tiles - 1) & 1, a.error, 44);
+        if (ok) ok = mbar_wait_warp(empty((tiles - 1) & 1), ((tiles - 1) >> 1) & 1, a.error, 44);
         tc_fence_after();
         if (ok) {
-            // accumulators of 64 rows lie in the first 16 lanes of each warp's 32.  Half a row goes through shared memory (free by now) and
-            // leaves as one bulk copy; rows 16 bytes more than their entries apart, so that lanes do not meet in the banks
-            const int r = DK == 128 ? quad * 32 + lane : quad * 16 + lane, c_lo = half * (DV / 2);
+            // accumulators of 64 rows lie in the first 16 lanes of each warp's 32
+            const int r = DK == 128 ? quad * 32 + lane : quad * 16 + lane, c_lo = (tid >> 7) * (DV / 2);
             const bool mine = r < p.dim && (DK == 128 || lane < 16);
-            uint8_t* stage = smem_raw + r * (DV * 4 + 16);
+            float4* u = reinterpret_cast<float4*>(p.work + at * p.dim * p.vdim) + r;
 #pragma unroll 1
             for (int c0 = c_lo; c0 < c_lo + DV / 2; c0 += 32) {
                 float o[32];
@@ -256,15 +283,8 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 if (mine) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<float4*>(stage + (c0 + i) * 4) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        if (c0 + i < p.vdim) u[(size_t)((c0 + i) >> 2) * p.dim] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 }
-            }
-            if (mine && c_lo < p.vdim) {
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.work + (at * p.dim + r) * p.vdim + c_lo),
-                             "r"(smem_u32(stage + c_lo * 4)), "r"(min(p.vdim - c_lo, DV / 2) * 4) : "memory");
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
             }
             if (tid == 0) p.seg_g[at] = (float)end;
         }
@@ -275,19 +295,21 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 }
 
 // ---- from segment to segment ------------------------------------------------------------------------------------------------
-// Four entries a thread.
+// Four entries a thread, a warp 8 rows of 16 columns: whole sectors of the states' order and of U's.
 __global__ void __launch_bounds__(256) hd_pass_tc_kernel(const HdTcArgs a) {
     pdl_sync();
     const HeadDecayArgs& p = a.p;
-    const int b = blockIdx.x, h = p.h0 + blockIdx.y, size = p.dim * p.vdim;
-    const int e = (blockIdx.z * 256 + threadIdx.x) * 4;
+    const int b = blockIdx.x, h = p.h0 + blockIdx.y, size = p.dim * p.vdim, across = (p.vdim + 15) / 16;
+    const int lane = threadIdx.x & 31, patch = blockIdx.z * 8 + (threadIdx.x >> 5), down = patch / across;
+    const int r = down * 8 + (lane & 7), c = (patch - down * across) * 16 + (lane >> 3) * 4;
     int t0, n, slot;
-    if (!hd_sequence(p, b, t0, n, slot) || e >= size) return;
+    if (!hd_sequence(p, b, t0, n, slot) || r >= p.dim || c >= p.vdim) return;
+    const int e = r * p.vdim + c;
     float S[4];
     dm_load<float, 4>(p.state + (size_t)slot * p.pitch + (size_t)h * size + e, S);
     const int segs = (n + p.seg - 1) / p.seg;
     const size_t first = (size_t)blockIdx.y * p.max_segs + t0 / p.seg + b;
-    const float* w = p.work + first * size + e;
+    const float* w = p.work + first * size + ((size_t)(c >> 2) * p.dim + r) * 4;
     __nv_bfloat16* st = a.starts + first * size + e;
     constexpr int U = 4;
     for (int i0 = 0; i0 < segs; i0 += U) {
@@ -369,6 +391,13 @@ __global__ void __launch_bounds__(HT_THREADS, VB == 4 ? 1 : 2)
 hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_s,
                   const __grid_constant__ CUtensorMap map_g, const HdTcArgs a) {
+    if (threadIdx.x == 0) {
+        ht_fetch_map(&map_q);
+        ht_fetch_map(&map_k);
+        ht_fetch_map(&map_v);
+        ht_fetch_map(&map_s);
+        if (a.p.gate) ht_fetch_map(&map_g);
+    }
     pdl_sync();
     constexpr int DK = KB * 64, DV = VB * 64;
     constexpr uint32_t BOX = HT_TILE * 128, K_BYTES = KB * BOX, V_BYTES = VB * BOX, S_BOX = DK * 128, TMEM_COLS = VB == 4 ? 512 : 256;
@@ -403,29 +432,27 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         mbar_init(g_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncwarp();
     if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
     const HdSegment s = hd_find(p, x);
     const int last = blockIdx.x - x * a.tiles;              // this block's tile of its segment
     const int q0 = s.t0 + last * HT_TILE, nq = min(HT_TILE, s.n - last * HT_TILE), kv = h / (p.H / p.G);     // nq <= 0: no such tile
+    // the first copies do not wait for the other warps: this one has made their barriers.  What v's place holds first is S_0
+    if (warp == 0 && nq > 0 && elect_one()) {
+        mbar_expect_tx(q_full, K_BYTES);
+        ht_load_tile<KB>(sq, &map_q, q_full, h, q0);
+        mbar_expect_tx(v_full, VB * S_BOX);
+#pragma unroll
+        for (int b = 0; b < VB; ++b) tma_load_3d(sv + b * S_BOX, &map_s, v_full, b * 64, 0, blockIdx.y * p.max_segs + x);
+        mbar_expect_tx(k_full, K_BYTES);
+        ht_load_tile<KB>(sk, &map_k, k_full, kv, s.t0);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_o = tmem_slot, tmem_s = tmem_slot + DV;
     if (nq <= 0) {
     } else if (warp == 0) {
-        // what v's place holds first is S_0
-        if (elect_one()) {
-            mbar_expect_tx(q_full, K_BYTES);
-#pragma unroll
-            for (int b = 0; b < KB; ++b) tma_load_3d(sq + b * BOX, &map_q, q_full, b * 64, h, q0);
-            mbar_expect_tx(v_full, VB * S_BOX);
-#pragma unroll
-            for (int b = 0; b < VB; ++b) tma_load_3d(sv + b * S_BOX, &map_s, v_full, b * 64, 0, blockIdx.y * p.max_segs + x);
-            mbar_expect_tx(k_full, K_BYTES);
-#pragma unroll
-            for (int b = 0; b < KB; ++b) tma_load_3d(sk + b * BOX, &map_k, k_full, b * 64, kv, s.t0);
-        }
-        __syncwarp();
         int k_issued = 1, v_issued = 1;
         bool ok = true, gate_issued = false;
         for (int j = 0; j <= last; ++j) {
@@ -433,8 +460,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             if (!ok) break;
             if (elect_one()) {
                 mbar_expect_tx(v_full, V_BYTES);
-#pragma unroll
-                for (int b = 0; b < VB; ++b) tma_load_3d(sv + b * BOX, &map_v, v_full, b * 64, kv, s.t0 + j * HT_TILE);
+                ht_load_tile<VB>(sv, &map_v, v_full, kv, s.t0 + j * HT_TILE);
             }
             __syncwarp();
             v_issued = j + 2;
@@ -444,8 +470,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             if (j == last) {
                 if (elect_one()) {
                     mbar_expect_tx(g_full, V_BYTES);
-#pragma unroll
-                    for (int b = 0; b < VB; ++b) tma_load_3d(sq + b * BOX, &map_g, g_full, b * 64, h, q0);
+                    ht_load_tile<VB>(sq, &map_g, g_full, h, q0);
                 }
                 __syncwarp();
                 gate_issued = true;
@@ -453,8 +478,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             }
             if (elect_one()) {
                 mbar_expect_tx(k_full, K_BYTES);
-#pragma unroll
-                for (int b = 0; b < KB; ++b) tma_load_3d(sk + b * BOX, &map_k, k_full, b * 64, kv, s.t0 + (j + 1) * HT_TILE);
+                ht_load_tile<KB>(sk, &map_k, k_full, kv, s.t0 + (j + 1) * HT_TILE);
             }
             __syncwarp();
             k_issued = j + 2;
@@ -678,13 +702,13 @@ template <int KB, int VB>
 static void ht_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& ms, const CUtensorMap& mg,
                       const HdTcArgs& a, cudaStream_t s) {
     const HeadDecayArgs& p = a.p;
-    const size_t box = (size_t)HT_TILE * 128, smem_u = ht_update_area(KB, VB) + 8 * 8 + sizeof(HtSums),
+    const size_t box = (size_t)HT_TILE * 128, smem_u = (2 * KB + VB) * box + 8 * 8 + sizeof(HtSums),
                  smem_r = ((2 * KB > VB ? 2 * KB : VB) + VB) * box + 12 * 8 + sizeof(HtRowsShared);
     static PerDevice allowed_u, allowed_r;
     tb_allow_smem(allowed_u, (const void*)hd_update_tc_kernel<KB, VB>, smem_u);
     tb_allow_smem(allowed_r, (const void*)hd_rows_tc_kernel<KB, VB>, smem_r);
     if (p.nt) TB_LAUNCH((hd_update_tc_kernel<KB, VB>), dim3(p.max_segs, p.heads), HT_THREADS, smem_u, s, mk, mv, a);
-    TB_LAUNCH((hd_pass_tc_kernel), dim3(p.B, p.heads, (p.dim * p.vdim / 4 + 255) / 256), 256, 0, s, a);
+    TB_LAUNCH((hd_pass_tc_kernel), dim3(p.B, p.heads, (p.dim / 8 * ((p.vdim + 15) / 16) + 7) / 8), 256, 0, s, a);
     if (p.nt) TB_LAUNCH((hd_rows_tc_kernel<KB, VB>), dim3(p.max_segs * a.tiles, p.heads), HT_THREADS, smem_r, s, mq, mk, mv, ms, mg, a);
 }
 
@@ -731,10 +755,10 @@ int tb_head_decay_tc_bf16(const void* q, const void* k, const void* v, const voi
     const int kb = (dim + 63) / 64, vb = vdim <= 64 ? 1 : vdim <= 128 ? 2 : 4;
     CUtensorMap mq, mk, mv, ms, mg = {};
     const int rows = nt > 0 ? nt : 1;
-    if (make_map_3d(&mq, q, dim, H, rows, dim, ldq, 1, HT_TILE) || make_map_3d(&mk, k, dim, G, rows, dim, ldk, 1, HT_TILE) ||
-        make_map_3d(&mv, v, vdim, G, rows, vdim, ldv, 1, HT_TILE) ||
+    if (make_map_3d(&mq, q, dim, H, rows, dim, ldq, 1, HT_HALF) || make_map_3d(&mk, k, dim, G, rows, dim, ldk, 1, HT_HALF) ||
+        make_map_3d(&mv, v, vdim, G, rows, vdim, ldv, 1, HT_HALF) ||
         make_map_3d(&ms, a.starts, vdim, dim, (long long)all, vdim, (long long)size, kb * 64, 1) ||
-        (gate && make_map_3d(&mg, gate, vdim, H, rows, vdim, ldgate, 1, HT_TILE)))
+        (gate && make_map_3d(&mg, gate, vdim, H, rows, vdim, ldgate, 1, HT_HALF)))
         return TB_ERR_UNSUPPORTED;
     for (p.h0 = 0; p.h0 < H; p.h0 += heads) {
         p.heads = H - p.h0 < heads ? H - p.h0 : heads;
