@@ -34,7 +34,7 @@ def _inputs(dtype, H, G, dim, vdim, lens, decay, gated, seed, slots=None, behind
     return d, more, torch.tensor([0] + list(lens)).cumsum(0).int().cuda()
 
 
-def _check(d, more, lens, new_state, dtype, tensor_cores, state0, scale=None):
+def _check(d, more, lens, new_state, dtype, tensor_cores, state0, scale=None, untouched=True):
     H, dim, vdim = d["q"].shape[1], d["q"].shape[2], d["v"].shape[2]
     scale = dim ** -0.5 if scale is None else scale
     at, f = 0, lambda t: t.double().cpu()
@@ -51,6 +51,8 @@ def _check(d, more, lens, new_state, dtype, tensor_cores, state0, scale=None):
         err = (f(new_state[slot]) - S).abs()
         assert bool((err <= state_bounds(M, dim, n, tensor_cores)).all()), (b, n, float((err / state_bounds(M, dim, n, tensor_cores)).max()))
         at += n
+    if not untouched:
+        return
     assert bool((d["out"][at:] == 7.0).all()), "rows behind the last sequence"
     named = set(d["slots"].tolist())
     for slot in set(range(state0.shape[0])) - named:
@@ -59,7 +61,7 @@ def _check(d, more, lens, new_state, dtype, tensor_cores, state0, scale=None):
 
 SHAPES = [  # H, G, dim, vdim
     (2, 2, 128, 128), (4, 2, 64, 64), (3, 1, 128, 64), (2, 1, 64, 128), (2, 2, 80, 96), (1, 1, 256, 256), (3, 3, 17, 33), (1, 1, 1, 1),
-    (2, 1, 128, 256), (2, 2, 96, 130)]
+    (2, 1, 128, 256), (2, 2, 96, 130), (2, 2, 8, 8), (2, 1, 16, 24), (2, 2, 72, 72), (1, 1, 40, 136)]
 
 
 @pytest.mark.parametrize("decay", ["input", "fixed", "strong"])
@@ -96,11 +98,13 @@ def test_steps(dtype, H, G, dim, vdim):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_a_long_sequence_in_pieces_and_whole(dtype):
     """2,500 tokens at once, in three prompts and the last few one by one: the same states and outputs, all within the bounds."""
+    from transformer_b200.csrc import lib
     from transformer_b200.parts import decay_attention, decay_attention_step
     H, G, dim, vdim, n = 2, 1, 128, 128, 2500
     d, more, starts = _inputs(dtype, H, G, dim, vdim, [n], "input", False, 3, slots=torch.tensor([1]))
     state0 = d["state"].clone()
     decay_attention(seq_start=starts, **d)
+    assert not lib.gemm_tc_status()
     _check(d, more, [n], d["state"], dtype, dtype == torch.bfloat16, state0)
     whole, d["state"] = d["out"].clone(), state0.clone()
     d["out"].fill_(7.0)
@@ -115,6 +119,7 @@ def test_a_long_sequence_in_pieces_and_whole(dtype):
 
 def test_many_sequences_and_portions_of_heads(monkeypatch):
     """150 short sequences (their segments are found 32 guesses at a time), with scratch for one head at a time: the same bits."""
+    from transformer_b200.csrc import lib
     from transformer_b200.parts import decay_attention, head_decay
     lens = [(3, 0, 70, 1, 130)[i % 5] for i in range(150)]
     for dtype in (torch.float32, torch.bfloat16):
@@ -124,9 +129,34 @@ def test_many_sequences_and_portions_of_heads(monkeypatch):
             d, more, starts = _inputs(dtype, 4, 2, 64, 64, lens, "input", True, 9)
             state0 = d["state"].clone()
             decay_attention(seq_start=starts, **d, **more)
+            assert not lib.gemm_tc_status()
             outs.append((d["out"].clone(), d["state"].clone()))
         _check(d, more, lens, d["state"], dtype, dtype == torch.bfloat16, state0)
         assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+@pytest.mark.parametrize("dim,vdim", [(128, 128), (64, 128), (128, 64), (128, 256), (64, 64)])
+def test_many_heads_behind_one_another(dim, vdim):
+    """More heads and sequences than the GPU has places for blocks: a block goes through several heads.  One head at a time has the same
+    bits; some are looked at in 64 bits."""
+    from transformer_b200.csrc import lib
+    from transformer_b200.parts import decay_attention
+    H, G, lens = 11, 11, [(1, 130, 300, 0, 257, 128)[i % 6] for i in range(100)]
+    d, more, starts = _inputs(torch.bfloat16, H, G, dim, vdim, lens, "input", True, 2)
+    state0 = d["state"].clone()
+    decay_attention(seq_start=starts, **d, **more)
+    assert not lib.gemm_tc_status()
+    out, state = d["out"].clone(), d["state"].clone()
+    d["state"].copy_(state0)
+    for h in range(H):
+        one = {n: d[n][:, h:h + 1] for n in ("q", "k", "v", "out")}
+        S = d["state"][:, h:h + 1].clone()
+        decay_attention(state=S, slots=d["slots"], seq_start=starts, log_decay=d["log_decay"][:, h:h + 1].contiguous(),
+                        norm=more["norm"][h:h + 1], gate=more["gate"][:, h:h + 1], eps=EPS, **one)
+        assert torch.equal(S, state[:, h:h + 1])
+    assert not lib.gemm_tc_status() and torch.equal(d["out"], out)
+    d["out"], d["state"] = out[: sum(lens[:6])], state
+    _check(d, {**more, "gate": more["gate"][: sum(lens[:6])]}, lens[:6], state, torch.bfloat16, True, state0, untouched=False)
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
