@@ -16,6 +16,36 @@
 #define HD_STEP_U 16
 #define HD_PAD 68               // pitch of a tile of 64 columns
 
+// ROWS x 64 entries of a block of 256 threads, all asked for before any is stored.
+template <int ROWS, typename Load, typename Store>
+__device__ __forceinline__ void hd_tile(Load load, Store store) {
+    float x[ROWS / 4];
+#pragma unroll
+    for (int u = 0; u < ROWS / 4; ++u) x[u] = load((int)(threadIdx.x >> 6) + 4 * u, (int)(threadIdx.x & 63));
+#pragma unroll
+    for (int u = 0; u < ROWS / 4; ++u) store((int)(threadIdx.x >> 6) + 4 * u, (int)(threadIdx.x & 63), x[u]);
+}
+// r += four entries of a row times four of another, 4 x 4 results a thread
+__device__ __forceinline__ void hd_fma16(const float* a_row, const float* b_row, F2 (&r)[4][2]) {
+    const float4 a = *reinterpret_cast<const float4*>(a_row), b = *reinterpret_cast<const float4*>(b_row);
+    const float av[4] = {a.x, a.y, a.z, a.w};
+    F2 b0, b1;
+    b0.f = make_float2(b.x, b.y);
+    b1.f = make_float2(b.z, b.w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        F2 x;
+        x.f = make_float2(av[i], av[i]);
+        r[i][0] = fma2(x, b0, r[i][0]);
+        r[i][1] = fma2(x, b1, r[i][1]);
+    }
+}
+__device__ __forceinline__ void hd_zero(F2 (&r)[4][2]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i][0].f = r[i][1].f = make_float2(0.f, 0.f);
+}
+__device__ __forceinline__ float hd_of(const F2 (&r)[4][2], int i, int l) { return l & 1 ? r[i][l >> 1].f.y : r[i][l >> 1].f.x; }
+
 // ---- U of a segment ----------------------------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(256) hd_update_kernel(const HeadDecayArgs p) {
@@ -33,24 +63,16 @@ __global__ void __launch_bounds__(256) hd_update_kernel(const HeadDecayArgs p) {
     const T* v = static_cast<const T*>(p.v) + (size_t)s.t0 * p.ldv + (size_t)kv * p.vdim;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const HdSum last = c[s.n - 1];
-    float acc[4][4] = {};
+    F2 acc[4][2];
+    hd_zero(acc);
     for (int j0 = 0; j0 < s.n; j0 += 32) {
-        for (int e = threadIdx.x; e < 32 * 64; e += 256) {
-            const int j = e >> 6, r = e & 63;
-            const bool in = j0 + j < s.n;
-            ks[j][r] = in && r0 + r < p.dim ? ldf(k + (size_t)(j0 + j) * p.ldk + r0 + r) * expf(hd_minus(last, c[j0 + j])) : 0.f;
-            vs[j][r] = in && c0 + r < p.vdim ? ldf(v + (size_t)(j0 + j) * p.ldv + c0 + r) : 0.f;
-        }
+        hd_tile<32>([&](int j, int r) { return j0 + j < s.n && r0 + r < p.dim ? ldf(k + (size_t)(j0 + j) * p.ldk + r0 + r) * expf(hd_minus(last, c[j0 + j])) : 0.f; },
+                    [&](int j, int r, float x) { ks[j][r] = x; });
+        hd_tile<32>([&](int j, int r) { return j0 + j < s.n && c0 + r < p.vdim ? ldf(v + (size_t)(j0 + j) * p.ldv + c0 + r) : 0.f; },
+                    [&](int j, int r, float x) { vs[j][r] = x; });
         __syncthreads();
 #pragma unroll 8
-        for (int j = 0; j < 32; ++j) {
-            const float4 a = *reinterpret_cast<const float4*>(&ks[j][ty * 4]), b = *reinterpret_cast<const float4*>(&vs[j][tx * 4]);
-            const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int l = 0; l < 4; ++l) acc[i][l] += av[i] * bv[l];
-        }
+        for (int j = 0; j < 32; ++j) hd_fma16(&ks[j][ty * 4], &vs[j][tx * 4], acc);
         __syncthreads();
     }
     const size_t at = (size_t)blockIdx.y * p.max_segs + blockIdx.x;
@@ -60,7 +82,7 @@ __global__ void __launch_bounds__(256) hd_update_kernel(const HeadDecayArgs p) {
 #pragma unroll
         for (int l = 0; l < 4; ++l) {
             const int r = r0 + ty * 4 + i, col = c0 + tx * 4 + l;
-            if (r < p.dim && col < p.vdim) u[(size_t)r * p.vdim + col] = acc[i][l];
+            if (r < p.dim && col < p.vdim) u[(size_t)r * p.vdim + col] = hd_of(acc, i, l);
         }
     if (blockIdx.z == 0 && threadIdx.x == 0) p.seg_g[at] = last.hi + last.lo;
 }
@@ -119,29 +141,20 @@ __global__ void __launch_bounds__(256) hd_rows_kernel(const HeadDecayArgs p) {
     const T* v = static_cast<const T*>(p.v) + (size_t)s.t0 * p.ldv + (size_t)kv * vdim;
     const float* S = p.work + ((size_t)blockIdx.y * p.max_segs + blockIdx.x) * dim * vdim;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    for (int e = threadIdx.x; e < HD_SEG * dim; e += 256) {
-        const int i = e / dim, r = e - i * dim;
-        q_s[r * HD_PAD + i] = i < s.n ? ldf(q + (size_t)i * p.ldq + r) : 0.f;
-    }
+    for (int d0 = 0; d0 < dim; d0 += 64)
+        hd_tile<HD_SEG>([&](int i, int r) { return i < s.n && d0 + r < dim ? ldf(q + (size_t)i * p.ldq + d0 + r) : 0.f; },
+                        [&](int i, int r, float x) { if (d0 + r < dim) q_s[(d0 + r) * HD_PAD + i] = x; });
     // scores, rows = queries ty * 4 .., columns = keys tx * 4 ..
-    float acc[4][4] = {};
-    auto fma16 = [&](const float* a_row, const float* b_row, float (&r)[4][4]) {
-        const float4 a = *reinterpret_cast<const float4*>(a_row + ty * 4), b = *reinterpret_cast<const float4*>(b_row + tx * 4);
-        const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int l = 0; l < 4; ++l) r[i][l] += av[i] * bv[l];
-    };
+    F2 acc[4][2];
+    hd_zero(acc);
     for (int d0 = 0; d0 < dim; d0 += 64) {
         const int here = min(64, dim - d0);
         __syncthreads();
-        for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-            const int j = e >> 6, r = e & 63;
-            if (r < here) x_s[r * HD_PAD + j] = j < s.n ? ldf(k + (size_t)j * p.ldk + d0 + r) : 0.f;
-        }
+        hd_tile<HD_SEG>([&](int j, int r) { return j < s.n && r < here ? ldf(k + (size_t)j * p.ldk + d0 + r) : 0.f; },
+                        [&](int j, int r, float x) { x_s[r * HD_PAD + j] = x; });
         __syncthreads();
-        for (int r = 0; r < here; ++r) fma16(q_s + (size_t)(d0 + r) * HD_PAD, x_s + r * HD_PAD, acc);
+#pragma unroll 4
+        for (int r = 0; r < here; ++r) hd_fma16(q_s + (size_t)(d0 + r) * HD_PAD + ty * 4, x_s + r * HD_PAD + tx * 4, acc);
     }
     // a query sees the keys up to its own; the others' weights are 0 and their values are not multiplied at all
 #pragma unroll
@@ -150,53 +163,57 @@ __global__ void __launch_bounds__(256) hd_rows_kernel(const HeadDecayArgs p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int qi = ty * 4 + i;
-            p_s[j * HD_PAD + qi] = j <= qi && qi < s.n ? acc[i][l] * expf(hd_minus(c[qi], c[j])) : 0.f;
+            p_s[j * HD_PAD + qi] = j <= qi && qi < s.n ? hd_of(acc, i, l) * expf(hd_minus(c[qi], c[j])) : 0.f;
         }
     }
     float from_start[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) from_start[i] = ty * 4 + i < s.n ? expf(c[ty * 4 + i].hi + c[ty * 4 + i].lo) : 0.f;
-    float o[TILES][4][4];
+    F2 o[TILES][4][2];
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
         const int c0 = t * 64;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int l = 0; l < 4; ++l) o[t][i][l] = 0.f;
+        hd_zero(o[t]);
         for (int d0 = 0; d0 < dim; d0 += 64) {
             const int here = min(64, dim - d0);
             __syncthreads();
-            for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-                const int r = e >> 6, col = e & 63;
-                if (r < here) x_s[r * HD_PAD + col] = c0 + col < vdim ? S[(size_t)(d0 + r) * vdim + c0 + col] : 0.f;
-            }
+            hd_tile<64>([&](int r, int col) { return r < here && c0 + col < vdim ? S[(size_t)(d0 + r) * vdim + c0 + col] : 0.f; },
+                        [&](int r, int col, float x) { x_s[r * HD_PAD + col] = x; });
             __syncthreads();
-            for (int r = 0; r < here; ++r) fma16(q_s + (size_t)(d0 + r) * HD_PAD, x_s + r * HD_PAD, o[t]);
+#pragma unroll 4
+            for (int r = 0; r < here; ++r) hd_fma16(q_s + (size_t)(d0 + r) * HD_PAD + ty * 4, x_s + r * HD_PAD + tx * 4, o[t]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int l = 0; l < 4; ++l) o[t][i][l] *= from_start[i];
-        __syncthreads();
-        for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-            const int j = e >> 6, col = e & 63;
-            x_s[j * HD_PAD + col] = j < s.n && c0 + col < vdim ? ldf(v + (size_t)j * p.ldv + c0 + col) : 0.f;
+        for (int i = 0; i < 4; ++i) {
+            F2 f;
+            f.f = make_float2(from_start[i], from_start[i]);
+            o[t][i][0] = mul2(o[t][i][0], f);
+            o[t][i][1] = mul2(o[t][i][1], f);
         }
         __syncthreads();
-        const int seen = min(s.n, ty * 4 + 4);
-        for (int j = 0; j < seen; ++j) {
-            if (j <= ty * 4) {
-                fma16(p_s + j * HD_PAD, x_s + j * HD_PAD, o[t]);
-            } else {
-                for (int i = j - ty * 4; i < 4; ++i)
+        hd_tile<HD_SEG>([&](int j, int col) { return j < s.n && c0 + col < vdim ? ldf(v + (size_t)j * p.ldv + c0 + col) : 0.f; },
+                        [&](int j, int col, float x) { x_s[j * HD_PAD + col] = x; });
+        __syncthreads();
+        // the keys that all four of this thread's rows see, and the last three one row after the other: a weight of 0 is not multiplied
+        // with a value that may be no number
+        const int whole = min(s.n, ty * 4 + 1);
+#pragma unroll 4
+        for (int j = 0; j < whole; ++j) hd_fma16(p_s + j * HD_PAD + ty * 4, x_s + j * HD_PAD + tx * 4, o[t]);
 #pragma unroll
-                    for (int l = 0; l < 4; ++l) {
-                        const float add = p_s[j * HD_PAD + ty * 4 + i] * x_s[j * HD_PAD + tx * 4 + l];
-                        if (i == 1) o[t][1][l] += add;
-                        if (i == 2) o[t][2][l] += add;
-                        if (i == 3) o[t][3][l] += add;
-                    }
+        for (int c1 = 1; c1 < 4; ++c1) {
+            const int j = ty * 4 + c1;
+            if (j >= s.n) break;
+            const float4 b = *reinterpret_cast<const float4*>(x_s + j * HD_PAD + tx * 4);
+            F2 b0, b1;
+            b0.f = make_float2(b.x, b.y);
+            b1.f = make_float2(b.z, b.w);
+#pragma unroll
+            for (int i = c1; i < 4; ++i) {
+                F2 w;
+                const float x = p_s[j * HD_PAD + ty * 4 + i];
+                w.f = make_float2(x, x);
+                o[t][i][0] = fma2(w, b0, o[t][i][0]);
+                o[t][i][1] = fma2(w, b1, o[t][i][1]);
             }
         }
     }
@@ -210,8 +227,8 @@ __global__ void __launch_bounds__(256) hd_rows_kernel(const HeadDecayArgs p) {
         for (int t = 0; t < TILES; ++t)
 #pragma unroll
             for (int l = 0; l < 4; ++l) {
-                o[t][i][l] *= p.scale;
-                sq += o[t][i][l] * o[t][i][l];
+                const float y = hd_of(o[t], i, l) * p.scale;
+                sq += y * y;
             }
 #pragma unroll
         for (int m = 8; m > 0; m >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, m);
@@ -223,7 +240,7 @@ __global__ void __launch_bounds__(256) hd_rows_kernel(const HeadDecayArgs p) {
             for (int l = 0; l < 4; ++l) {
                 const int col = t * 64 + tx * 4 + l;
                 if (col >= vdim) continue;
-                float y = o[t][i][l];
+                float y = hd_of(o[t], i, l) * p.scale;
                 if (p.gate) {
                     const float z = ldf(gate + (size_t)qi * p.ldgate + col);
                     y = y * rs * p.norm[(size_t)h * vdim + col] * (z / (1.0f + expf(-z)));

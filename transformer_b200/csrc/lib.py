@@ -11,6 +11,7 @@ there is no CPU path and no library fallback behind these functions.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from typing import Dict
 
@@ -519,11 +520,13 @@ def split_delta_record_size(dim: int) -> int:
     return library().tb_split_delta_record_size(dim)
 
 
+@functools.lru_cache(maxsize=4096)
 def head_decay_segments(tokens: int, sequences: int) -> int:
     """Segments that a step's tokens are cut into at most, for the linear attention with one decay a head."""
     return library().tb_head_decay_segments(tokens, sequences)
 
 
+@functools.lru_cache(maxsize=4096)
 def head_decay_tc_work(tokens: int, sequences: int, dim: int, vdim: int, tiles: int) -> int:
     """Floats of scratch a head for the tcgen05 kernels of that attention, with segments of ``tiles`` times 128 tokens; 0: they do not
     take such heads."""

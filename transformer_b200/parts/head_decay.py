@@ -47,7 +47,7 @@ def _states(t, name, H, dim, vdim):
     return max(s[0], H * dim * vdim)
 
 
-def _checked(q, k, v, log_decay, state, slots, out, norm, gate, new_state):
+def _checked(q, k, v, log_decay, state, slots, out, norm, gate, new_state, seq_start=None):
     """The sizes and distances that both operators hand to their kernels."""
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k and v are [tokens, heads, entries]")
@@ -83,10 +83,18 @@ def _checked(q, k, v, log_decay, state, slots, out, norm, gate, new_state):
         ldgate = _rows(gate, "gate", nt, H, vdim, dtype)
         if norm.dtype != torch.float32 or norm.numel() != H * vdim or not norm.is_contiguous():
             raise ValueError(f"norm: a contiguous float32 tensor of [{H}, {vdim}], got {norm.dtype} {tuple(norm.shape)}")
-    lib.check_device(q, k, v, log_decay, state, slots, out, norm, gate, new_state)
+    lib.check_device(q, k, v, log_decay, state, slots, out, norm, gate, new_state, seq_start)
     head = (q.data_ptr(), k.data_ptr(), v.data_ptr(), lib.ptr(gate), *lds, ldgate, log_decay.data_ptr(), g_stride, lib.ptr(norm),
             state.data_ptr(), new_state.data_ptr(), pitch, new_pitch, out.data_ptr(), ldo)
     return head, (H, G, dim, vdim, state.shape[0])
+
+
+def _work(per, H, q, scratch):
+    """So many heads as WORK_BYTES holds of ``per`` floats each, and the scratch for them."""
+    heads = max(1, min(H, WORK_BYTES // (4 * max(per, 1))))
+    if scratch is None:
+        return heads, torch.empty(heads * per, dtype=torch.float32, device=q.device)
+    return heads, scratch("head_decay.work", (heads * per,), torch.float32)
 
 
 def decay_attention(q, k, v, log_decay, state, seq_start, slots, out, *, scale=None, norm=None, gate=None, eps=1e-6, new_state=None,
@@ -100,27 +108,21 @@ def decay_attention(q, k, v, log_decay, state, seq_start, slots, out, *, scale=N
     behind the last sequence, and states that no sequence names, are left alone, as is all of a sequence whose bounds or slot lie
     outside the tensors.  A sequence without tokens keeps its state.  What is no number in v stays in its channel, behind its
     token.  ``scratch(name, shape, dtype)``: where the workspace comes from (default: allocated by the call)."""
-    head, sizes = _checked(q, k, v, log_decay, state, slots, out, norm, gate, new_state)
     B, nt = slots.shape[0], q.shape[0]
-    if seq_start.dtype != torch.int32 or tuple(seq_start.shape) != (B + 1,) or not seq_start.is_contiguous():
+    if seq_start.dtype != torch.int32 or seq_start.shape != (B + 1,) or not seq_start.is_contiguous():
         raise ValueError(f"seq_start must be a contiguous int32 tensor of {B + 1} entries")
-    lib.check_device(q, seq_start)
-    H, G, dim, vdim, n_slots = sizes
+    head, sizes = _checked(q, k, v, log_decay, state, slots, out, norm, gate, new_state, seq_start)
+    H, _, dim, vdim, _ = sizes
     more = (*sizes, dim ** -0.5 if scale is None else float(scale), float(eps))
-
-    def work(per):          # scratch for so many heads as WORK_BYTES holds
-        heads = max(1, min(H, WORK_BYTES // (4 * max(per, 1))))
-        n = heads * per
-        return heads, torch.empty(n, dtype=torch.float32, device=q.device) if scratch is None else scratch("head_decay.work", (n,), torch.float32)
-
+    rows = (seq_start.data_ptr(), slots.data_ptr())
     per = lib.head_decay_tc_work(nt, B, dim, vdim, TILES) if q.dtype == torch.bfloat16 and USE_TC else 0
     if per:
-        heads, w = work(per)
-        if lib.try_call("tb_head_decay_tc_bf16", *head, seq_start.data_ptr(), slots.data_ptr(), w.data_ptr(), TILES, heads, nt, B, *more):
+        heads, work = _work(per, H, q, scratch)
+        if lib.try_call("tb_head_decay_tc_bf16", *head, *rows, work.data_ptr(), TILES, heads, nt, B, *more):
             return
     segments = lib.head_decay_segments(nt, B)
-    heads, w = work(segments * (dim * vdim + 1))
-    lib.call("tb_head_decay_" + lib.suffix(q.dtype), *head, seq_start.data_ptr(), slots.data_ptr(), w.data_ptr(), segments, heads, nt, B, *more)
+    heads, work = _work(segments * (dim * vdim + 1), H, q, scratch)
+    lib.call("tb_head_decay_" + lib.suffix(q.dtype), *head, *rows, work.data_ptr(), segments, heads, nt, B, *more)
 
 
 def decay_attention_step(q, k, v, log_decay, state, slots, out, *, scale=None, norm=None, gate=None, eps=1e-6, new_state=None) -> None:
