@@ -76,23 +76,28 @@ struct HdSum {
 };
 __device__ __forceinline__ float hd_minus(HdSum a, HdSum b) { return (a.hi - b.hi) + (a.lo - b.lo); }
 
-// c_i for the n tokens from t0 on, by the first warp; the others wait at the caller's barrier.  In 64 bits.
+// c_i for the n <= 64 tokens from t0 on, by the first warp; the others wait at the caller's barrier.  In 64 bits.
 __device__ __forceinline__ void hd_sums(const HeadDecayArgs& p, int h, int t0, int n, HdSum* c) {
     if (threadIdx.x >= 32) return;
     const int lane = threadIdx.x;
-    double before = 0.0;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-        const int i = i0 + lane;
-        double x = i < n ? (double)hd_log_decay(p.g[(size_t)(p.g_stride ? t0 + i : 0) * p.g_stride + h]) : 0.0;
+    float g[2];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double u = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += u;
+    for (int u = 0; u < 2; ++u) g[u] = p.g[(size_t)(p.g_stride ? t0 + min(lane + 32 * u, n - 1) : 0) * p.g_stride + h];
+    double x[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) x[u] = lane + 32 * u < n ? (double)hd_log_decay(g[u]) : 0.0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const double v = __shfl_up_sync(0xffffffffu, x[u], o);
+            if (lane >= o) x[u] += v;
         }
-        x += before;
-        before = __shfl_sync(0xffffffffu, x, 31);
-        const float hi = (float)x;
-        if (i < n) c[i] = HdSum{hi, (float)(x - (double)hi)};
+    x[1] += __shfl_sync(0xffffffffu, x[0], 31);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const float hi = (float)x[u];
+        if (lane + 32 * u < n) c[lane + 32 * u] = HdSum{hi, (float)(x[u] - (double)hi)};
     }
 }
 

@@ -367,20 +367,25 @@ __global__ void __launch_bounds__(256) hd_pass_tc_kernel(const HdTcArgs a) {
     int t0, n, slot;
     if (!hd_sequence(p, b, t0, n, slot) || r >= p.dim || c >= p.vdim) return;
     const int e = r * p.vdim + c;
+    auto once = [](const float* at, float (&f)[4]) {         // read here for the last time
+        const float4 x = __ldcs(reinterpret_cast<const float4*>(at));
+        f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
+    };
     float S[4];
-    dm_load<float, 4>(p.state + (size_t)slot * p.pitch + (size_t)h * size + e, S);
+    once(p.state + (size_t)slot * p.pitch + (size_t)h * size + e, S);
     const int segs = (n + p.seg - 1) / p.seg;
     const size_t first = (size_t)blockIdx.y * p.max_segs + t0 / p.seg + b;
-    const float* w = p.work + first * size + ((size_t)(c >> 2) * p.dim + r) * 4;
-    __nv_bfloat16* st = a.starts + first * size + e;
-    constexpr int U = 4;
+    const float* __restrict__ w = p.work + first * size + ((size_t)(c >> 2) * p.dim + r) * 4;
+    const float* __restrict__ gs = p.seg_g + first;
+    __nv_bfloat16* __restrict__ st = a.starts + first * size + e;
+    constexpr int U = 8;            // segments asked for together: with one sequence of few heads the walk is bound by their latency
     for (int i0 = 0; i0 < segs; i0 += U) {
         float u[U][4], d[U];
 #pragma unroll
         for (int i = 0; i < U; ++i)
             if (i0 + i < segs) {
-                dm_load<float, 4>(w + (size_t)(i0 + i) * size, u[i]);
-                d[i] = p.seg_g[first + i0 + i];
+                once(w + (size_t)(i0 + i) * size, u[i]);
+                d[i] = gs[i0 + i];
             }
 #pragma unroll
         for (int i = 0; i < U; ++i)
@@ -393,7 +398,7 @@ __global__ void __launch_bounds__(256) hd_pass_tc_kernel(const HdTcArgs a) {
                 for (int l = 0; l < 4; ++l) S[l] = S[l] * f + u[i][l];
             }
     }
-    dm_store<4>(p.new_state + (size_t)slot * p.new_pitch + (size_t)h * size + e, S);
+    __stcs(reinterpret_cast<float4*>(p.new_state + (size_t)slot * p.new_pitch + (size_t)h * size + e), make_float4(S[0], S[1], S[2], S[3]));
 }
 
 // ---- outputs -------------------------------------------------------------------------------------------------------------------

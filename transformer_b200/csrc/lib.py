@@ -138,7 +138,7 @@ class TapeMap(ctypes.Structure):
     _fields_ = [("base", ctypes.c_ulonglong), ("size", ctypes.c_ulonglong), ("delta", ctypes.c_longlong)]
 
 
-_NO_STREAM = {"tb_head_decay_segments": "ii",
+_NO_STREAM = {"tb_head_decay_segments": "iiii",
               "tb_decay_scan_rect_record_size": "ii", "tb_split_delta_record_size": "i",
               "tb_decay_state_size": "iii", "tb_decay_record_size": "i",
               "tb_attention_window_mma_tile_tokens": "ii", "tb_delta_state_size": "iiiii", "tb_delta_record_size": "i", "tb_delta_scan_lanes": "i", "tb_delta_chunk_record_size": "iii", "tb_delta_chunk_tokens": "", "tb_delta_value_pitch": "i", "tb_mlstm_state_size": "ii", "tb_mlstm_parallel_size": "iiii", "tb_mlstm_parallel_gates": "", "tb_mlstm_parallel_tokens": "", "tb_latent_attention_tile_tokens": "i", "tb_latent_tc_tile_tokens": "iii", "tb_attention_tile_tokens": "ii", "tb_gemm_tc_takes_pairs": "iiiiiii", "tb_gemm_tc_status": "", "tb_attention_prefill_tile_tokens": "",
@@ -521,9 +521,10 @@ def split_delta_record_size(dim: int) -> int:
 
 
 @functools.lru_cache(maxsize=4096)
-def head_decay_segments(tokens: int, sequences: int) -> int:
-    """Segments that a step's tokens are cut into at most, for the linear attention with one decay a head."""
-    return library().tb_head_decay_segments(tokens, sequences)
+def head_decay_segments(tokens: int, sequences: int, dim: int, vdim: int) -> int:
+    """Segments that a step's tokens are cut into at most, for the linear attention with one decay a head; 0: so few tokens and small
+    heads that one kernel does all without scratch."""
+    return library().tb_head_decay_segments(tokens, sequences, dim, vdim)
 
 
 @functools.lru_cache(maxsize=4096)

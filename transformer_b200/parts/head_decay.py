@@ -115,12 +115,15 @@ def decay_attention(q, k, v, log_decay, state, seq_start, slots, out, *, scale=N
     H, _, dim, vdim, _ = sizes
     more = (*sizes, dim ** -0.5 if scale is None else float(scale), float(eps))
     rows = (seq_start.data_ptr(), slots.data_ptr())
+    segments = lib.head_decay_segments(nt, B, dim, vdim)
+    if segments == 0:               # few tokens, small heads: one kernel does all
+        lib.call("tb_head_decay_" + lib.suffix(q.dtype), *head, *rows, 0, 0, 1, nt, B, *more)
+        return
     per = lib.head_decay_tc_work(nt, B, dim, vdim, TILES) if q.dtype == torch.bfloat16 and USE_TC else 0
     if per:
         heads, work = _work(per, H, q, scratch)
         if lib.try_call("tb_head_decay_tc_bf16", *head, *rows, work.data_ptr(), TILES, heads, nt, B, *more):
             return
-    segments = lib.head_decay_segments(nt, B)
     heads, work = _work(segments * (dim * vdim + 1), H, q, scratch)
     lib.call("tb_head_decay_" + lib.suffix(q.dtype), *head, *rows, work.data_ptr(), segments, heads, nt, B, *more)
 
