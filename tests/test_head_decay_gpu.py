@@ -185,6 +185,63 @@ def test_what_is_no_number_stays_behind_its_token(dtype, dim, vdim, bad):
     assert torch.equal(good_S, got_S)
 
 
+def test_what_is_no_number_in_a_gated_row():
+    """With the norm a row of a head that has one is none as a whole; the rows before it and the other head keep their bits."""
+    from transformer_b200.parts import decay_attention
+    n, at, outs = 400, 150, []
+    for value in (0.5, float("inf")):
+        d, more, starts = _inputs(torch.bfloat16, 2, 2, 128, 128, [n], "input", True, 1)
+        d["state"].zero_()
+        d["v"][at, 0, 5] = value
+        decay_attention(seq_start=starts, **d, **more)
+        outs.append(d["out"][:n].float().cpu())
+    good, got = outs
+    assert bool(torch.isfinite(good).all()) and not bool(torch.isfinite(got[at:, 0]).any())
+    got[at:, 0] = good[at:, 0]
+    assert torch.equal(good, got)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim,vdim", [(128, 128), (64, 64), (17, 33)])
+def test_no_tokens_and_no_sequences(dtype, dim, vdim):
+    from transformer_b200.parts import decay_attention, decay_attention_step
+    d, _, starts = _inputs(dtype, 2, 1, dim, vdim, [0, 0, 0], "input", False, 1, behind=0)
+    new = torch.full_like(d["state"], 5.0)
+    decay_attention(seq_start=starts, new_state=new, **d)
+    for slot in range(5):
+        assert torch.equal(new[slot], d["state"][slot] if slot in d["slots"].tolist() else torch.full_like(new[slot], 5.0))
+    before = new.clone()
+    none = dict(d, slots=d["slots"][:0])
+    decay_attention(seq_start=starts[:1], new_state=new, **none)
+    decay_attention_step(new_state=new, **none)
+    assert torch.equal(new, before)
+
+
+@pytest.mark.parametrize("shift,pitch", [(1, 0), (0, 3), (4, 4)])
+@pytest.mark.parametrize("dim,vdim", [(128, 128), (64, 64), (24, 40)])
+def test_rows_that_are_not_whole_16_byte_pieces(dim, vdim, shift, pitch):
+    """bfloat16 rows that begin anywhere, an odd distance apart, and states with a slot pitch: what the TMA copies do not take."""
+    from transformer_b200.parts import decay_attention, decay_attention_step
+    H, lens = 2, [70, 3, 129]
+    d, more, starts = _inputs(torch.bfloat16, H, H, dim, vdim, lens, "input", True, 8)
+    for n in ("q", "k", "v", "out"):
+        wide = torch.zeros(d[n].shape[0], H * d[n].shape[2] + 16 + pitch, dtype=torch.bfloat16, device="cuda")
+        view = wide[:, shift:shift + H * d[n].shape[2]].unflatten(1, (H, -1))
+        view.copy_(d[n])
+        d[n] = view
+    wide = torch.zeros(d["state"].shape[0], H * dim * vdim + pitch, device="cuda")
+    state = wide[:, :H * dim * vdim].unflatten(1, (H, dim, vdim))
+    state.copy_(d["state"])
+    state0, d["state"] = d["state"], state
+    decay_attention(seq_start=starts, **d, **more)
+    _check(d, more, lens, d["state"], torch.bfloat16, True, state0)
+    state.copy_(state0)
+    d["out"].fill_(7.0)
+    cut = {n: d[n][:3] for n in ("q", "k", "v", "log_decay", "out")}
+    decay_attention_step(state=d["state"], slots=d["slots"], norm=more["norm"], gate=more["gate"][:3], eps=EPS, **cut)
+    _check({**d, **cut}, {**more, "gate": more["gate"][:3]}, [1, 1, 1], d["state"], torch.bfloat16, False, state0)
+
+
 def test_sequences_whose_numbers_are_out_of_range_are_left_alone():
     """Bounds and slots outside the tensors: nothing of those sequences is read or written, the others are done."""
     from transformer_b200.parts import decay_attention, decay_attention_step

@@ -357,7 +357,8 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 }
 
 // ---- from segment to segment ------------------------------------------------------------------------------------------------
-// Four entries a thread, a warp 8 rows of 16 columns: whole sectors of the states' order and of U's.
+// Four entries a thread, a warp 8 rows of 16 columns: whole sectors of the states' order and of U's.  U: segments asked for together.
+template <int U>
 __global__ void __launch_bounds__(256) hd_pass_tc_kernel(const HdTcArgs a) {
     pdl_sync();
     const HeadDecayArgs& p = a.p;
@@ -378,7 +379,6 @@ __global__ void __launch_bounds__(256) hd_pass_tc_kernel(const HdTcArgs a) {
     const float* __restrict__ w = p.work + first * size + ((size_t)(c >> 2) * p.dim + r) * 4;
     const float* __restrict__ gs = p.seg_g + first;
     __nv_bfloat16* __restrict__ st = a.starts + first * size + e;
-    constexpr int U = 8;            // segments asked for together: with one sequence of few heads the walk is bound by their latency
     for (int i0 = 0; i0 < segs; i0 += U) {
         float u[U][4], d[U];
 #pragma unroll
@@ -858,7 +858,11 @@ static void ht_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtens
     tb_allow_smem(allowed_u, (const void*)hd_update_tc_kernel<KB, VB>, smem_u);
     tb_allow_smem(allowed_r, (const void*)hd_rows_tc_kernel<KB, VB>, smem_r);
     if (p.nt) TB_LAUNCH((hd_update_tc_kernel<KB, VB>), dim3(p.max_segs, (p.heads + a.heads_u - 1) / a.heads_u), HT_THREADS, smem_u, s, mk, mv, a);
-    TB_LAUNCH((hd_pass_tc_kernel), dim3(p.B, p.heads, (p.dim / 8 * ((p.vdim + 15) / 16) + 7) / 8), 256, 0, s, a);
+    // one wave of blocks is bound by the latency of its loads, more by memory: us of the whole call with 8 and 4 at a time, 8,192 tokens of 16
+    // heads of 128 87 and 99, 2,048 of 32 49.9 and 51.1, 11,875 in 11 sequences of 32 237 and 226
+    const dim3 grid(p.B, p.heads, (p.dim / 8 * ((p.vdim + 15) / 16) + 7) / 8);
+    if ((long long)grid.x * grid.y * grid.z <= 148 * 8) TB_LAUNCH((hd_pass_tc_kernel<8>), grid, 256, 0, s, a);
+    else TB_LAUNCH((hd_pass_tc_kernel<4>), grid, 256, 0, s, a);
     if (p.nt) TB_LAUNCH((hd_rows_tc_kernel<KB, VB>), dim3(p.max_segs * a.tiles, (p.heads + a.heads_r - 1) / a.heads_r), HT_THREADS, smem_r, s, mq, mk, mv, ms, mg, mo, a);
 }
 

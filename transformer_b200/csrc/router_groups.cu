@@ -146,7 +146,7 @@ __device__ __noinline__ int rg_choose64(const RouterGroupArgs& p, const float* r
 }
 
 template <int PER>
-__global__ void __launch_bounds__(RG_WARPS * 32) router_groups_kernel(const RouterGroupArgs p) {
+__global__ void __launch_bounds__(RG_WARPS * 32) router_groups_kernel(const __grid_constant__ RouterGroupArgs p) {
     extern __shared__ float rg_sm[];        // [RG_WARPS][E + E / 32 + 1] where groups' worths are found
     pdl_sync();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -245,6 +245,11 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_groups_kernel(const Rout
             again = least - most <= 4.f * loose + 2.5e-7f * (fabsf(least) + fabsf(most));
         }
         const unsigned kept = __ballot_sync(0xffffffffu, in);
+        if (size % PER == 0) {          // a lane's experts are of one group
+            if (!(kept >> ((int)((e0 + 0.5f) * per_size) * L & 31) & 1u))
+#pragma unroll
+                for (int i = 0; i < PER; ++i) key[i] = 0u;
+        } else
 #pragma unroll
         for (int i = 0; i < PER; ++i)
             if (!(kept >> ((int)((e0 + i + 0.5f) * per_size) * L & 31) & 1u)) key[i] = 0u;
@@ -276,11 +281,12 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_groups_kernel(const Rout
             const unsigned best = __reduce_max_sync(0xffffffffu, key[0]);
             const int from = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
             const int e = __shfl_sync(0xffffffffu, e0 + (int)(places & 15u), from);
-            const bool taken = lane == from;
+            if (lane == from) {
 #pragma unroll
-            for (int i = 0; i + 1 < PER; ++i) key[i] = taken ? key[i + 1] : key[i];
-            key[PER - 1] = taken ? 0u : key[PER - 1];
-            places = taken ? places >> 4 : places;
+                for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1];
+                key[PER - 1] = 0u;
+                places >>= 4;
+            }
             if (lane == j) {
                 my_key = best;
                 mine = e;

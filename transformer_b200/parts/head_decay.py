@@ -20,7 +20,7 @@ from .linear import matmul_nt
 MOST_DIM = 256                  # entries of a head, key or value
 USE_TC = True                   # bfloat16 prompts: the tcgen05 kernels, for the heads that they take
 TILES = 2                       # tiles of 128 tokens in one of their segments
-WORK_BYTES = 512 << 20          # the most scratch for the segments' states: of more heads than it holds, portions are done in turn
+WORK_BYTES = 256 << 20          # the most scratch for the segments' states: of more heads than it holds, portions are done in turn
 
 
 def _rows(t, name, nt, heads, dim, dtype):
