@@ -34,8 +34,8 @@ def bounds(o, size, dtype, dim, n, tensor_cores):
 
 
 def state_bounds(M, dim, n, tensor_cores):
-    """On the tensor cores a weighted key is two bfloat16s: what is left of it is 2^-8 of 2^-8."""
-    return M * ((512 + n // 32 + 16) * F32 + (BF16 * BF16 if tensor_cores else 0.0)) + 1e-30
+    """On the tensor cores a weighted key is three bfloat16s: what is left of it is 2^-8 of 2^-8 of 2^-8, and a third of the additions more."""
+    return M * ((512 + n // 32 + 16) * F32 * (3 if tensor_cores else 1) + (BF16 ** 3 if tensor_cores else 0.0)) + 1e-30
 
 
 def normed(o, off, norm, gate, eps, dtype):

@@ -6,8 +6,8 @@
 //   hd_rows_tc_kernel     a block = 128 tokens of a segment x a head: O = e^{c_i} (Q S_0), then += P V for each 128 keys up to its own,
 //                         P = (Q K^T) e^{c_i - c_j}; with a gate the heads' norm at the end
 //
-// The states stay in float: K' is written as two bfloat16s, the value and what its rounding left (over K and beside it), and both are multiplied
-// with V into the same accumulator, so U is off by 2^-16 of its terms.  P and S_0 enter products whose results are rounded to bfloat16 anyway, and
+// The states stay in float: K' is written as three bfloat16s, the value and what its rounding left twice (over K and beside it), and all are
+// multiplied with V into the same accumulator, so U has float's error (with two of them 2.8e-6 of its norm, measured).  P and S_0 enter products whose results are rounded to bfloat16 anyway, and
 // are rounded to it themselves.
 // A factor e^{c_i - c_j} is one exponential for a row and 32 keys times one for a key and the end of its 32, both at most 1; inside
 // the 32 x 32 on the diagonal, where the first would grow, one exponential each.  P takes its place over the scores in tensor memory (the A
@@ -167,8 +167,9 @@ __device__ __forceinline__ void ht_sums(const HeadDecayArgs& p, int n, int tid, 
 }
 
 // ---- U of a segment -----------------------------------------------------------------------------------------------------
-// A block takes its segment's heads one after the other, 64 keys at a time in two stages: copies and decays run ahead into the next
-// head, and a head's U leaves while the next one's keys are multiplied (two accumulators).  U has its entries in the order
+// A block takes its segment's heads one after the other, 64 keys at a time: copies (two stages of K and V) and decays run ahead into the
+// next head, and a head's U leaves while the next one's keys are multiplied (two accumulators).  What rounding left of K' has room for
+// one stage, so the next keys are weighted when the product before them is done.  U has its entries in the order
 // [vdim / 4][dim][4]: a warp's 32 rows of four columns are 512 bytes on end.
 template <int KB, int VB>
 __global__ void __launch_bounds__(HT_THREADS, VB == 4 ? 1 : 2)
@@ -179,11 +180,12 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
     pdl_sync();
     constexpr int DK = KB * 64, DV = VB * 64;
-    constexpr uint32_t BOX = HT_HALF * 128, K_BYTES = KB * BOX, V_BYTES = VB * BOX, STAGE = 2 * K_BYTES + V_BYTES, TMEM_COLS = 2 * DV;
-    extern __shared__ __align__(1024) uint8_t smem_raw[];       // a stage: K (then K'), what rounding left of K', V
+    constexpr uint32_t BOX = HT_HALF * 128, K_BYTES = KB * BOX, V_BYTES = VB * BOX, STAGE = K_BYTES + V_BYTES, TMEM_COLS = 2 * DV;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];       // two stages of K (then K') and V; what one and two roundings left of K'
     const HeadDecayArgs& p = a.p;
     const uint32_t base = smem_u32(smem_raw);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + 2 * STAGE);
+    uint8_t* rest = smem_raw + 2 * STAGE;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(rest + 2 * K_BYTES);
     HtSums* sums = reinterpret_cast<HtSums*>(bars + 12);        // by the head's parity
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 11);
     const int warp = warp_number(), lane = threadIdx.x & 31;
@@ -216,7 +218,7 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     auto copy = [&](int it) {
         const int i = it / tiles, t = s.t0 + (it - i * tiles) * HT_HALF, kv = (p.h0 + at0 + i) / (p.H / p.G);
         if (elect_one()) {
-            const uint32_t sk = base + (it & 1) * STAGE, sv = sk + 2 * K_BYTES;
+            const uint32_t sk = base + (it & 1) * STAGE, sv = sk + K_BYTES;
             mbar_expect_tx(full(it & 1), K_BYTES + V_BYTES);
 #pragma unroll
             for (int b = 0; b < KB; ++b) tma_load_3d(sk + b * BOX, &map_k, full(it & 1), b * 64, kv, t);
@@ -252,12 +254,13 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint32_t sk = base + (it & 1) * STAGE, sv = sk + 2 * K_BYTES, to = tmem + (i & 1) * DV;
+                    const uint32_t sk = base + (it & 1) * STAGE, sv = sk + K_BYTES, sr = base + 2 * STAGE, to = tmem + (i & 1) * DV;
                     const int ks = (min(HT_HALF, s.n - j * HT_HALF) + 15) / 16;
                     for (int k = 0; k < ks; ++k) {
                         const uint64_t dv = ht_desc(sv + k * 2048, BOX);
                         umma_bf16(to, ht_desc(sk + k * 2048, BOX), dv, idesc, (j | k) != 0);
-                        umma_bf16(to, ht_desc(sk + K_BYTES + k * 2048, BOX), dv, idesc, 1);
+                        umma_bf16(to, ht_desc(sr + k * 2048, BOX), dv, idesc, 1);
+                        umma_bf16(to, ht_desc(sr + K_BYTES + k * 2048, BOX), dv, idesc, 1);
                     }
                     umma_commit(empty(it & 1));
                     if (j == tiles - 1) umma_commit(u_full(i & 1));
@@ -306,40 +309,44 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             const double end = sum.before[(s.n + 31) / 32];
             for (int j = 0; j < tiles; ++j, ++it) {
                 ok = ok && mbar_wait_warp(full(it & 1), (it >> 1) & 1, a.error, 43);
+                if (it > 0) ok = ok && mbar_wait_warp(empty(~it & 1), ((it - 1) >> 1) & 1, a.error, 43);
                 if (!ok) continue;
                 const int token = j * HT_HALF + key;
                 const bool there = token < s.n;
                 const float w = there ? expf(sum.e[token] + (float)(end - sum.before[(token >> 5) + 1])) : 0.f;
                 F2 w2;
                 w2.f = make_float2(w, w);
-                uint8_t* row = smem_raw + (it & 1) * STAGE + key * 128;
+                uint8_t *row = smem_raw + (it & 1) * STAGE + key * 128, *left = rest + key * 128;
                 // four threads a key, a quarter of its 16-byte pieces each
 #pragma unroll
                 for (int c = 0; c < 2 * KB; ++c) {
                     const int piece = part * 2 * KB + c;
-                    uint4* here = reinterpret_cast<uint4*>(row + (piece >> 3) * BOX + (((piece & 7) ^ (key & 7)) << 4));
+                    const int offset = (piece >> 3) * BOX + (((piece & 7) ^ (key & 7)) << 4);
+                    uint4* here = reinterpret_cast<uint4*>(row + offset);
                     const uint4 raw = there ? *here : make_uint4(0u, 0u, 0u, 0u);
                     const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
-                    uint32_t hi[4], lo[4];
+                    uint32_t part3[3][4];       // the value, and what is left of it twice
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        F2 f, g;
+                        F2 f;
                         f.f = make_float2(__uint_as_float(in[e] << 16), __uint_as_float(in[e] & 0xffff0000u));
                         f = mul2(f, w2);
-                        const __nv_bfloat162 r = __floats2bfloat162_rn(f.f.x, f.f.y);
-                        hi[e] = *reinterpret_cast<const uint32_t*>(&r);
-                        g.f = make_float2(f.f.x - __uint_as_float(hi[e] << 16), f.f.y - __uint_as_float(hi[e] & 0xffff0000u));
-                        const __nv_bfloat162 q = __floats2bfloat162_rn(g.f.x, g.f.y);
-                        lo[e] = *reinterpret_cast<const uint32_t*>(&q);
+#pragma unroll
+                        for (int r = 0; r < 3; ++r) {
+                            const __nv_bfloat162 q = __floats2bfloat162_rn(f.f.x, f.f.y);
+                            part3[r][e] = *reinterpret_cast<const uint32_t*>(&q);
+                            f.f = make_float2(f.f.x - __uint_as_float(part3[r][e] << 16), f.f.y - __uint_as_float(part3[r][e] & 0xffff0000u));
+                        }
                     }
-                    *here = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(here) + K_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    *here = make_uint4(part3[0][0], part3[0][1], part3[0][2], part3[0][3]);
+                    *reinterpret_cast<uint4*>(left + offset) = make_uint4(part3[1][0], part3[1][1], part3[1][2], part3[1][3]);
+                    *reinterpret_cast<uint4*>(left + K_BYTES + offset) = make_uint4(part3[2][0], part3[2][1], part3[2][2], part3[2][3]);
                 }
                 if (!there) {           // another sequence's values: 0 times one that is no number would not be 0
 #pragma unroll
                     for (int c = 0; c < 2 * VB; ++c) {
                         const int piece = part * 2 * VB + c;
-                        *reinterpret_cast<uint4*>(row + 2 * K_BYTES + (piece >> 3) * BOX + (piece & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4*>(row + K_BYTES + (piece >> 3) * BOX + (piece & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -852,6 +859,7 @@ static void ht_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtens
                       const CUtensorMap& mo, const HdTcArgs& a, cudaStream_t s) {
     const HeadDecayArgs& p = a.p;
     constexpr int WIDE = KB > VB ? KB : VB;
+    // the update: K's and V's boxes of half the rows in two stages, and K's twice for what rounding left
     const size_t box = (size_t)HT_TILE * 128, smem_u = (2 * KB + VB) * box + 12 * 8 + 2 * sizeof(HtSums),
                  smem_r = 3 * WIDE * box + 16 * 8 + sizeof(HtRowsShared);
     static PerDevice allowed_u, allowed_r;
