@@ -7,12 +7,12 @@
 //                         P = (Q K^T) e^{c_i - c_j}; with a gate the heads' norm at the end
 //
 // The states stay in float: K' is written as three bfloat16s, the value and what its rounding left twice (over K and beside it), and all are
-// multiplied with V into the same accumulator, so U has float's error (with two of them 2.8e-6 of its norm, measured).  P and S_0 enter products whose results are rounded to bfloat16 anyway, and
-// are rounded to it themselves.
+// multiplied with V into the same accumulator, so U has float's error (with two of them 2.8e-6 of its norm, measured).  P and S_0 enter
+// products whose results are rounded to bfloat16 anyway, and are rounded to it themselves.
 // A factor e^{c_i - c_j} is one exponential for a row and 32 keys times one for a key and the end of its 32, both at most 1; inside
 // the 32 x 32 on the diagonal, where the first would grow, one exponential each.  P takes its place over the scores in tensor memory (the A
 // operand of the second product).  Copies by TMA (3-D maps [tokens, heads, entries]: entries behind a head's are zeros), products issued
-// by one warp, four warps for the rows; two blocks an SM hide each other's waits.  Every wait is bounded.
+// by one warp, eight warps for the rows, two blocks an SM.  Every wait is bounded.
 #include <algorithm>
 
 #include "head_decay.cuh"
@@ -21,7 +21,7 @@
 
 #define HT_TILE 128
 #define HT_HALF 64              // rows of a TMA box, and keys that the update takes together
-#define HT_MOST 4               // tiles of a segment
+#define HT_MOST 2               // most tiles of a segment
 #define HT_WORKERS 256          // eight warps: two for each 32 lanes of tensor memory, half of the columns each
 #define HT_THREADS (64 + HT_WORKERS)
 #define HT_LOG2E 1.4426950408889634f
@@ -915,8 +915,9 @@ int tb_head_decay_tc_bf16(const void* q, const void* k, const void* v, const voi
     a.error = tc_error_ptr();
     if (!a.error) return tb_last_error();
     // Heads a block: the next one's copies run ahead, but longer blocks leave the SMs less evenly.  Up to four, where three rounds of blocks
-    // over their places (two an SM) remain.  us, 1, 2 and 4 heads, of the update / of the rows: 11,875 tokens in 11 sequences of 32 heads of 128
-    // 251.8, 246.9 and 258.3 / 251.8, 245.5 and 245.9; 8,192 of 16 103.6, 102.1 and 107.3 / 103.6, 103.3 and 105.2; 2,048 of 32 54.2, 56.1, 65.6 / 54.2, 53.9, 68.0
+    // over their places (two an SM) remain.  us of a call, 1, 2 and 4 heads a block of the update (with 2 of the rows) / of the rows (with 1 of
+    // the update): 11,875 tokens in 11 sequences of 32 heads of 128 245, 242 and 257 / 253, 245 and 245; 8,192 of 16 90.4, 88.5 and
+    // 94.3 / 91.2, 90.4 and 89.7; 2,048 of 32 50.9, 54.3 and 66.9 / 51.1, 50.9 and 64.1
     const long long places = 2 * 148;
     auto per_block = [&](long long blocks) { return (int)std::max(1LL, std::min({4LL, (long long)heads, blocks * heads / (3 * places)})); };
     a.heads_u = per_block(p.max_segs);

@@ -25,26 +25,29 @@ WORK_BYTES = 256 << 20          # the most scratch for the segments' states: of 
 
 def _rows(t, name, nt, heads, dim, dtype):
     """The distance of the rows of ``t`` [nt, heads, dim], whose heads lie one behind the other."""
-    if t.shape != (nt, heads, dim) or t.dtype != dtype:
+    if t.shape != (nt, heads, dim) or t.dtype is not dtype:
         raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, expected {dtype} {(nt, heads, dim)}")
-    s = t.stride()
-    if s[2] == 1 and s[1] == dim and s[0] >= heads * dim:
-        return s[0]
-    if (s[2] != 1 and dim > 1) or (s[1] != dim and heads > 1) or (s[0] < heads * dim and nt > 1):
-        raise ValueError(f"{name}: a row's heads must lie one behind the other, rows apart, got strides {s}")
-    return s[0] if nt > 1 else heads * dim
+    row, head, entry = t.stride()
+    if entry == 1 and head == dim and row >= heads * dim:
+        return row
+    # what the stride of an axis of one is does not matter
+    if (entry != 1 and dim > 1) or (head != dim and heads > 1) or (row < heads * dim and nt > 1):
+        raise ValueError(f"{name}: a row's heads must lie one behind the other, rows apart, got strides {t.stride()}")
+    return row if nt > 1 else heads * dim
 
 
 def _states(t, name, H, dim, vdim):
-    if t.dim() != 4 or t.shape[1:] != (H, dim, vdim) or t.dtype != torch.float32:
+    """The distance of the slots of ``t`` [slots, H, dim, vdim], float, each contiguous."""
+    if t.dim() != 4 or t.shape[1:] != (H, dim, vdim) or t.dtype is not torch.float32:
         raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)}, expected float32 [slots, {H}, {dim}, {vdim}]")
-    s = t.stride()
-    if s[3] == 1 and s[2] == vdim and s[1] == dim * vdim and s[0] >= H * s[1]:
-        return s[0]
-    if t.numel() and ((s[3] != 1 and vdim > 1) or (s[2] != vdim and dim > 1) or (s[1] != dim * vdim and H > 1) or
-                      (s[0] < H * dim * vdim and t.shape[0] > 1)):
-        raise ValueError(f"{name}: a slot's state must be contiguous, slots apart, got strides {s}")
-    return max(s[0], H * dim * vdim)
+    size = dim * vdim
+    slot, head, row, entry = t.stride()
+    if entry == 1 and row == vdim and head == size and slot >= H * size:
+        return slot
+    if t.numel() and ((entry != 1 and vdim > 1) or (row != vdim and dim > 1) or (head != size and H > 1) or
+                      (slot < H * size and t.shape[0] > 1)):
+        raise ValueError(f"{name}: a slot's state must be contiguous, slots apart, got strides {t.stride()}")
+    return max(slot, H * size)
 
 
 def _checked(q, k, v, log_decay, state, slots, out, norm, gate, new_state, seq_start=None):
@@ -52,41 +55,40 @@ def _checked(q, k, v, log_decay, state, slots, out, norm, gate, new_state, seq_s
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k and v are [tokens, heads, entries]")
     nt, H, dim = q.shape
-    G, vdim = k.shape[1], v.shape[2]
-    dtype = q.dtype
-    if dtype not in (torch.bfloat16, torch.float32):
+    G, vdim, dtype = k.shape[1], v.shape[2], q.dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise ValueError(f"kernels exist for float32 and bfloat16, not {dtype}")
     if G <= 0 or H <= 0 or H % G:
         raise ValueError(f"{H} heads cannot share the keys and values of {G}")
     if not (0 < dim <= MOST_DIM and 0 < vdim <= MOST_DIM):
         raise ValueError(f"heads have 1..{MOST_DIM} entries, got {dim} and {vdim}")
-    lds = (_rows(q, "q", nt, H, dim, dtype), _rows(k, "k", nt, G, dim, dtype), _rows(v, "v", nt, G, vdim, dtype))
+    ldq, ldk, ldv = _rows(q, "q", nt, H, dim, dtype), _rows(k, "k", nt, G, dim, dtype), _rows(v, "v", nt, G, vdim, dtype)
     ldo = _rows(out, "out", nt, H, vdim, dtype)
-    if log_decay.dtype != torch.float32 or (log_decay.shape != (nt, H) and log_decay.shape != (H,)) or \
-            (log_decay.stride(-1) != 1 and H > 1) or (log_decay.dim() == 2 and nt > 1 and log_decay.stride(0) < H):
+    each, strides = log_decay.shape == (nt, H), log_decay.stride()
+    if log_decay.dtype is not torch.float32 or not (each or log_decay.shape == (H,)) or (strides[-1] != 1 and H > 1) or \
+            (each and nt > 1 and strides[0] < H):
         raise ValueError(f"log_decay: float32 [{H}] or [{nt}, {H}] with contiguous rows, got {log_decay.dtype} {tuple(log_decay.shape)}")
-    g_stride = 0 if log_decay.dim() == 1 else max(log_decay.stride(0), H)
-    pitch = _states(state, "state", H, dim, vdim)
-    new_pitch = pitch
+    pitch = new_pitch = _states(state, "state", H, dim, vdim)
+    n_slots = state.shape[0]
     if new_state is None:
         new_state = state
     elif new_state is not state:
         new_pitch = _states(new_state, "new_state", H, dim, vdim)
-        if new_state.shape[0] != state.shape[0]:
-            raise ValueError(f"new_state has {new_state.shape[0]} slots, state {state.shape[0]}")
-    if slots.dtype != torch.int32 or slots.dim() != 1 or not slots.is_contiguous():
+        if new_state.shape[0] != n_slots:
+            raise ValueError(f"new_state has {new_state.shape[0]} slots, state {n_slots}")
+    if slots.dtype is not torch.int32 or slots.dim() != 1 or not slots.is_contiguous():
         raise ValueError("slots must be a contiguous int32 tensor")
     if (norm is None) != (gate is None):
         raise ValueError("a norm and a gate go together")
-    ldgate = 0
+    ldgate = p_gate = p_norm = 0
     if gate is not None:
-        ldgate = _rows(gate, "gate", nt, H, vdim, dtype)
-        if norm.dtype != torch.float32 or norm.numel() != H * vdim or not norm.is_contiguous():
+        ldgate, p_gate, p_norm = _rows(gate, "gate", nt, H, vdim, dtype), gate.data_ptr(), norm.data_ptr()
+        if norm.dtype is not torch.float32 or norm.numel() != H * vdim or not norm.is_contiguous():
             raise ValueError(f"norm: a contiguous float32 tensor of [{H}, {vdim}], got {norm.dtype} {tuple(norm.shape)}")
     lib.check_device(q, k, v, log_decay, state, slots, out, norm, gate, new_state, seq_start)
-    head = (q.data_ptr(), k.data_ptr(), v.data_ptr(), lib.ptr(gate), *lds, ldgate, log_decay.data_ptr(), g_stride, lib.ptr(norm),
-            state.data_ptr(), new_state.data_ptr(), pitch, new_pitch, out.data_ptr(), ldo)
-    return head, (H, G, dim, vdim, state.shape[0])
+    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), p_gate, ldq, ldk, ldv, ldgate, log_decay.data_ptr(),
+            max(strides[0], H) if each else 0, p_norm, state.data_ptr(), new_state.data_ptr(), pitch, new_pitch, out.data_ptr(),
+            ldo), (H, G, dim, vdim, n_slots)
 
 
 def _work(per, H, q, scratch):

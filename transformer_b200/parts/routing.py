@@ -6,6 +6,8 @@
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from ..csrc import lib
@@ -14,7 +16,8 @@ MOST_EXPERTS, MOST_CHOSEN, MOST_GROUPS = 1024, 30, 32       # of the kernel (csr
 SCORES = ("softmax", "sigmoid")
 
 
-def check_choice(experts: int, k: int, *, scores="softmax", groups=1, groups_use=1, group_top=1) -> None:
+@functools.lru_cache(maxsize=1024)
+def check_choice(experts: int, k: int, scores="softmax", groups=1, groups_use=1, group_top=1) -> None:
     """ValueError unless ``k`` of ``experts`` can be chosen in this way."""
     if scores not in SCORES:
         raise ValueError(f"scores are {' or '.join(SCORES)}, got {scores!r}")
@@ -41,15 +44,16 @@ def choose_experts(logits, index, weights, *, scores="softmax", bias=None, group
     spreads to the weights that it enters.  A row's indices always differ.  What is decided on sums of scores, or on scores and a
     bias, is what 64 bits decide."""
     nt, E = logits.shape
+    row, entry = logits.stride()
     k = index.shape[-1]
-    check_choice(E, k, scores=scores, groups=groups, groups_use=groups_use, group_top=group_top)
-    if logits.dtype != torch.float32 or (logits.stride(1) != 1 and E > 1) or (nt > 1 and logits.stride(0) < E):
+    check_choice(E, k, scores, groups, groups_use, group_top)
+    if logits.dtype is not torch.float32 or (entry != 1 and E > 1) or (nt > 1 and row < E):
         raise ValueError("the choice reads float32 logits with contiguous rows")
-    if index.shape != (nt, k) or weights.shape != (nt, k) or index.dtype != torch.int32 or \
-            weights.dtype != torch.float32 or not index.is_contiguous() or not weights.is_contiguous():
+    if index.shape != (nt, k) or weights.shape != (nt, k) or index.dtype is not torch.int32 or \
+            weights.dtype is not torch.float32 or not index.is_contiguous() or not weights.is_contiguous():
         raise ValueError(f"index (int32) and weights (float32) must be contiguous [{nt}, {k}] tensors")
-    if bias is not None and (bias.shape != (E,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
+    if bias is not None and (bias.shape != (E,) or bias.dtype is not torch.float32 or not bias.is_contiguous()):
         raise ValueError(f"the bias must be a contiguous float32 tensor of {E} entries")
     lib.check_device(logits, index, weights, bias)
-    lib.call("tb_router_groups", logits.data_ptr(), max(logits.stride(0), E), lib.ptr(bias), index.data_ptr(), weights.data_ptr(),
+    lib.call("tb_router_groups", logits.data_ptr(), max(row, E), lib.ptr(bias), index.data_ptr(), weights.data_ptr(),
              nt, E, k, groups, groups_use, group_top, scores == "softmax", bool(renorm), float(scale))
