@@ -19,7 +19,8 @@ from .linear import matmul_nt
 
 MOST_DIM = 256                  # entries of a head, key or value
 USE_TC = True                   # bfloat16 prompts: the tcgen05 kernels, for the heads that they take
-TILES = 2                       # tiles of 128 tokens in one of their segments
+TILES = 2                       # tiles of 128 tokens in one of their segments: with 1 and 2, 2,048 tokens of 32 heads 60 and 51 us, 11,875 in 11
+                                # sequences 299 and 241 (twice the states' way through memory); 4 left the SMs with few long blocks
 WORK_BYTES = 256 << 20          # the most scratch for the segments' states: of more heads than it holds, portions are done in turn
 
 
