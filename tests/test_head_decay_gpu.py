@@ -318,3 +318,26 @@ def test_captured_and_replayed_and_on_another_stream(dtype):
         fresh(seed)
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(result(), want[seed - 1]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_distances_that_pass_32_bits(dtype):
+    """Rows of decays, and slots, more than 2^31 floats apart: the bits of the same numbers side by side."""
+    from transformer_b200.parts import decay_attention, decay_attention_step
+    H, dim, vdim, far = 2, 72, 72, 2 ** 31 + 8
+    d, _, starts = _inputs(dtype, H, H, dim, vdim, [1, 1], "input", False, 1)
+    near = {k: v[:2] if k in ("q", "k", "v", "log_decay") else v for k, v in d.items()}
+    near["slots"], near["out"] = torch.tensor([1, 0], dtype=torch.int32, device="cuda"), torch.empty((2, H, vdim), dtype=dtype, device="cuda")
+    near["state"] = torch.randn((2, H, dim, vdim), device="cuda")
+    room = torch.empty(2 * far, device="cuda")                  # 17 GB, of which a few kilobytes are touched
+    g = room.as_strided((2, H), (far, 1), 0)
+    g.copy_(near["log_decay"])
+    for go in (lambda x: decay_attention(seq_start=starts, **x), lambda x: decay_attention_step(**x)):
+        state = room.as_strided((2, H, dim, vdim), (far, dim * vdim, vdim, 1), 1024)
+        state.copy_(near["state"])
+        apart = dict(near, log_decay=g, state=state, out=torch.empty_like(near["out"]))
+        here = dict(near, state=near["state"].clone())
+        go(here)
+        go(apart)
+        assert torch.equal(here["out"], apart["out"]) and torch.equal(here["state"], apart["state"])
+        assert not torch.equal(here["state"], near["state"])

@@ -46,6 +46,20 @@ def test_wide_heads_are_refused():
         decay_attention_step(**_args(vdim=260, B=6))
 
 
+def test_more_rows_than_32_bits_count():
+    """Of tensors that take no memory (on "meta")."""
+    n, meta = 2 ** 31, lambda *s, dt=F: torch.empty(s, dtype=dt, device="meta")
+    few = dict(q=meta(4, 1, 1), k=meta(4, 1, 1), v=meta(4, 1, 1), log_decay=meta(1), state=meta(n, 1, 1, 1), slots=meta(4, dt=torch.int32), out=meta(4, 1, 1))
+    many = dict(few, q=meta(n, 1, 1), k=meta(n, 1, 1), v=meta(n, 1, 1), out=meta(n, 1, 1), state=meta(4, 1, 1, 1))
+    for d in (few, many):
+        with pytest.raises(ValueError, match="at most"):
+            decay_attention(seq_start=meta(5, dt=torch.int32), **d)
+        with pytest.raises(ValueError, match="at most"):
+            decay_attention_step(**d)
+    with pytest.raises(ValueError, match="at most"):
+        choose_experts(meta(n, 1), meta(n, 1, dt=torch.int32), meta(n, 1))
+
+
 LOGITS = dict(logits=torch.zeros(5, 16), index=torch.zeros(5, 4, dtype=torch.int32), weights=torch.zeros(5, 4))
 
 

@@ -559,7 +559,7 @@ int tb_head_decay_rates(const float* a, const float* rate, const float* bias, fl
 
 #define TB_HEAD_DECAY(SFX, T)                                                                                              \
     int tb_head_decay_##SFX(const void* q, const void* k, const void* v, const void* gate, long long ldq, long long ldk,   \
-                            long long ldv, long long ldgate, const float* g, int g_stride, const float* norm,              \
+                            long long ldv, long long ldgate, const float* g, long long g_stride, const float* norm,        \
                             const float* state, float* new_state, long long pitch, long long new_pitch, void* out,         \
                             long long ldo, const int* seq_start, const int* slots, float* work, int max_segs, int heads,   \
                             int nt, int B, int H, int G, int dim, int vdim, int n_slots, float scale, float eps,           \
@@ -569,7 +569,7 @@ int tb_head_decay_rates(const float* a, const float* rate, const float* bias, fl
                                                  H, G, dim, vdim, n_slots, max_segs, HD_SEG, 0, H, scale, eps}, heads, s); \
     }                                                                                                                      \
     int tb_head_decay_step_##SFX(const void* q, const void* k, const void* v, const void* gate, long long ldq,             \
-                                 long long ldk, long long ldv, long long ldgate, const float* g, int g_stride,             \
+                                 long long ldk, long long ldv, long long ldgate, const float* g, long long g_stride,       \
                                  const float* norm, const float* state, float* new_state, long long pitch,                 \
                                  long long new_pitch, void* out, long long ldo, const int* slots, int B, int H, int G,     \
                                  int dim, int vdim, int n_slots, float scale, float eps, cudaStream_t s) {                 \

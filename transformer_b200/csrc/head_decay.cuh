@@ -25,7 +25,7 @@ struct HeadDecayArgs {
     float* work;                    // [heads of a portion][max_segs][dim][vdim]: U, then S_0
     float* seg_g;                   // [heads of a portion][max_segs]: c_L
     long long ldq, ldk, ldv, ldgate, ldo, pitch, new_pitch;
-    int g_stride;                   // 0: one row of decays for all tokens
+    long long g_stride;             // 0: one row of decays for all tokens
     int nt, B, H, G, dim, vdim, n_slots, max_segs, seg;
     int h0, heads;                  // the portion's first head and its heads
     float scale, eps;

@@ -894,7 +894,7 @@ long long tb_head_decay_tc_work(int nt, int B, int dim, int vdim, int tiles) {
 }
 
 int tb_head_decay_tc_bf16(const void* q, const void* k, const void* v, const void* gate, long long ldq, long long ldk, long long ldv,
-                          long long ldgate, const float* g, int g_stride, const float* norm, const float* state, float* new_state,
+                          long long ldgate, const float* g, long long g_stride, const float* norm, const float* state, float* new_state,
                           long long pitch, long long new_pitch, void* out, long long ldo, const int* seq_start, const int* slots,
                           float* work, int tiles, int heads, int nt, int B, int H, int G, int dim, int vdim, int n_slots, float scale,
                           float eps, cudaStream_t s) {

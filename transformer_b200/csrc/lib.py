@@ -113,9 +113,9 @@ _SIGNATURES: Dict[str, str] = {
     "tb_embed_learned_f32": "pppppiifppp", "tb_embed_learned_bf16": "pppppiifppp",
     "tb_post_add_layernorm_router_f32": "pppppippfipppfipiippppiii",
     "tb_post_add_layernorm_router_bf16": "pppppippfipppfipiippppiii",
-    "tb_head_decay_f32": "ppppllllpipppllplpppiiiiiiiiiff", "tb_head_decay_bf16": "ppppllllpipppllplpppiiiiiiiiiff",
-    "tb_head_decay_step_f32": "ppppllllpipppllplpiiiiiiff", "tb_head_decay_step_bf16": "ppppllllpipppllplpiiiiiiff",
-    "tb_head_decay_tc_bf16": "ppppllllpipppllplpppiiiiiiiiiff",
+    "tb_head_decay_f32": "ppppllllplpppllplpppiiiiiiiiiff", "tb_head_decay_bf16": "ppppllllplpppllplpppiiiiiiiiiff",
+    "tb_head_decay_step_f32": "ppppllllplpppllplpiiiiiiff", "tb_head_decay_step_bf16": "ppppllllplpppllplpiiiiiiff",
+    "tb_head_decay_tc_bf16": "ppppllllplpppllplpppiiiiiiiiiff",
     "tb_head_decay_rates": "ppppii",
     "tb_router_groups": "plpppiiiiiiiif",
 }
@@ -199,16 +199,6 @@ launch_count = 0     # launchers called so far (a launcher may start more than o
 _scope_stream = None  # inside stream_scope(): the handle of the stream that was current at its start
 
 
-# The handle of torch's current stream.  Without the Stream object that torch.cuda.current_stream() makes a look-up costs 0.3 us, with it 3.3.
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
-def _current_stream() -> int:
-    if _raw_stream is None:
-        return torch.cuda.current_stream().cuda_stream
-    return _raw_stream(torch.cuda.current_device())
-
-
 class stream_scope:
     """``with stream_scope():`` looks torch's current stream up once for all the launches inside (a model's forward
     pass is some hundred launches, and the look-up costs as much as a launch).  Whoever opens it must not
@@ -217,7 +207,7 @@ class stream_scope:
     def __enter__(self):
         global _scope_stream
         self._before = _scope_stream
-        _scope_stream = _current_stream()
+        _scope_stream = torch.cuda.current_stream().cuda_stream
         return self
 
     def __exit__(self, *exc):
@@ -227,7 +217,18 @@ class stream_scope:
 
 
 def _stream() -> int:
-    return _scope_stream if _scope_stream is not None else _current_stream()
+    return _scope_stream if _scope_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def operator_stream() -> int:
+    """The stream of an operator that is called by itself, outside a scope as a rule: without the Stream object that
+    torch.cuda.current_stream() makes a look-up costs 0.3 us, with it 3.3.  For the ``stream`` of :func:`call`."""
+    if _scope_stream is not None or _raw_stream is None:
+        return _stream()
+    return _raw_stream(torch.cuda.current_device())
 
 
 _recorder = None      # while a layer's calls are recorded: an object with launch(name, args) and foreign(kind, *tensors)
@@ -293,12 +294,12 @@ def foreign(kind: str, *tensors) -> None:
         _recorder.foreign(kind, *tensors)
 
 
-def try_call(name: str, *args) -> bool:
+def try_call(name: str, *args, stream=None) -> bool:
     """Like :func:`call`, but a kernel that refuses the sizes (TB_ERR_UNSUPPORTED) answers False
     instead of raising, so the caller can take the general kernel."""
     global launch_count
     fn = getattr(_lib if _lib is not None else library(), name)
-    rc = fn(*args, _stream()) if _timing is None else _timed(name, fn, args)
+    rc = fn(*args, _stream() if stream is None else stream) if _timing is None else _timed(name, fn, args)
     if rc == -2:
         return False
     if rc != 0:
@@ -309,12 +310,12 @@ def try_call(name: str, *args) -> bool:
     return True
 
 
-def call(name: str, *args) -> None:
-    """Launch ``name`` on torch's current stream."""
+def call(name: str, *args, stream=None) -> None:
+    """Launch ``name`` on torch's current stream (``stream``: its handle, where the caller has looked it up)."""
     global launch_count
     launch_count += 1
     fn = getattr(_lib if _lib is not None else library(), name)
-    rc = fn(*args, _stream()) if _timing is None else _timed(name, fn, args)
+    rc = fn(*args, _stream() if stream is None else stream) if _timing is None else _timed(name, fn, args)
     if rc != 0:
         raise KernelError(f"{name}: {_error_text(rc)}")
     if _recorder is not None:

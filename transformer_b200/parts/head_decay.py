@@ -18,6 +18,7 @@ from .base import MIXERS, Mixer, ParamDecl, StateNeed
 from .linear import matmul_nt
 
 MOST_DIM = 256                  # entries of a head, key or value
+MOST_ROWS = 2 ** 31 - 1         # tokens, sequences, slots: the kernels count them in 32 bits
 USE_TC = True                   # bfloat16 prompts: the tcgen05 kernels, for the heads that they take
 TILES = 2                       # tiles of 128 tokens in one of their segments: with 1 and 2, 2,048 tokens of 32 heads 60 and 51 us, 11,875 in 11
                                 # sequences 299 and 241 (twice the states' way through memory); 4 left the SMs with few long blocks
@@ -77,6 +78,8 @@ def _checked(q, k, v, log_decay, state, slots, out, norm, gate, new_state, seq_s
         new_pitch = _states(new_state, "new_state", H, dim, vdim)
         if new_state.shape[0] != n_slots:
             raise ValueError(f"new_state has {new_state.shape[0]} slots, state {n_slots}")
+    if max(nt, n_slots, slots.numel()) > MOST_ROWS:
+        raise ValueError(f"{nt} tokens, {slots.numel()} sequences, {n_slots} slots: at most {MOST_ROWS} of each")
     if slots.dtype is not torch.int32 or slots.dim() != 1 or not slots.is_contiguous():
         raise ValueError("slots must be a contiguous int32 tensor")
     if (norm is None) != (gate is None):
@@ -107,7 +110,8 @@ def decay_attention(q, k, v, log_decay, state, seq_start, slots, out, *, scale=N
 
     q [nt, H, dim], k [nt, G, dim], v [nt, G, vdim], gate and out [nt, H, vdim] (bfloat16 or float32, all of one type) may be
     slices of wider rows; ``log_decay`` float [nt, H] or [H], a value above 0 counts as 0; ``norm`` float [H, vdim]; ``scale``
-    defaults to dim^-1/2.  The states afterwards go to ``new_state`` (same rows; default: ``state`` itself).  Rows of ``out``
+    defaults to dim^-1/2.  The states afterwards go to ``new_state`` (same rows; default: ``state`` itself).  Neither that nor ``out`` may
+    overlap anything else that the call reads.  Rows of ``out``
     behind the last sequence, and states that no sequence names, are left alone, as is all of a sequence whose bounds or slot lie
     outside the tensors.  A sequence without tokens keeps its state.  What is no number in v stays in its channel, behind its
     token.  ``scratch(name, shape, dtype)``: where the workspace comes from (default: allocated by the call)."""
@@ -117,18 +121,18 @@ def decay_attention(q, k, v, log_decay, state, seq_start, slots, out, *, scale=N
     head, sizes = _checked(q, k, v, log_decay, state, slots, out, norm, gate, new_state, seq_start)
     H, _, dim, vdim, _ = sizes
     more = (*sizes, dim ** -0.5 if scale is None else float(scale), float(eps))
-    rows = (seq_start.data_ptr(), slots.data_ptr())
+    rows, stream = (seq_start.data_ptr(), slots.data_ptr()), lib.operator_stream()
     segments = lib.head_decay_segments(nt, B, dim, vdim)
     if segments == 0:               # few tokens, small heads: one kernel does all
-        lib.call("tb_head_decay_" + lib.suffix(q.dtype), *head, *rows, 0, 0, 1, nt, B, *more)
+        lib.call("tb_head_decay_" + lib.suffix(q.dtype), *head, *rows, 0, 0, 1, nt, B, *more, stream=stream)
         return
     per = lib.head_decay_tc_work(nt, B, dim, vdim, TILES) if q.dtype == torch.bfloat16 and USE_TC else 0
     if per:
         heads, work = _work(per, H, q, scratch)
-        if lib.try_call("tb_head_decay_tc_bf16", *head, *rows, work.data_ptr(), TILES, heads, nt, B, *more):
+        if lib.try_call("tb_head_decay_tc_bf16", *head, *rows, work.data_ptr(), TILES, heads, nt, B, *more, stream=stream):
             return
     heads, work = _work(segments * (dim * vdim + 1), H, q, scratch)
-    lib.call("tb_head_decay_" + lib.suffix(q.dtype), *head, *rows, work.data_ptr(), segments, heads, nt, B, *more)
+    lib.call("tb_head_decay_" + lib.suffix(q.dtype), *head, *rows, work.data_ptr(), segments, heads, nt, B, *more, stream=stream)
 
 
 def decay_attention_step(q, k, v, log_decay, state, slots, out, *, scale=None, norm=None, gate=None, eps=1e-6, new_state=None) -> None:
@@ -137,7 +141,7 @@ def decay_attention_step(q, k, v, log_decay, state, slots, out, *, scale=None, n
     if slots.shape[0] != q.shape[0]:
         raise ValueError(f"{q.shape[0]} tokens but {slots.shape[0]} slots")
     lib.call("tb_head_decay_step_" + lib.suffix(q.dtype), *head, slots.data_ptr(), slots.shape[0], *sizes,
-             sizes[2] ** -0.5 if scale is None else float(scale), float(eps))
+             sizes[2] ** -0.5 if scale is None else float(scale), float(eps), stream=lib.operator_stream())
 
 
 @MIXERS.register("head_decay")

@@ -12,6 +12,7 @@ import torch
 
 from ..csrc import lib
 
+MOST_TOKENS = 2 ** 31 - 1
 MOST_EXPERTS, MOST_CHOSEN, MOST_GROUPS = 1024, 30, 32       # of the kernel (csrc/router_groups.cu)
 SCORES = ("softmax", "sigmoid")
 
@@ -47,6 +48,8 @@ def choose_experts(logits, index, weights, *, scores="softmax", bias=None, group
     row, entry = logits.stride()
     k = index.shape[-1]
     check_choice(E, k, scores, groups, groups_use, group_top)
+    if nt > MOST_TOKENS:
+        raise ValueError(f"{nt} tokens, at most {MOST_TOKENS}")
     if logits.dtype is not torch.float32 or (entry != 1 and E > 1) or (nt > 1 and row < E):
         raise ValueError("the choice reads float32 logits with contiguous rows")
     if index.shape != (nt, k) or weights.shape != (nt, k) or index.dtype is not torch.int32 or \
@@ -56,4 +59,5 @@ def choose_experts(logits, index, weights, *, scores="softmax", bias=None, group
         raise ValueError(f"the bias must be a contiguous float32 tensor of {E} entries")
     lib.check_device(logits, index, weights, bias)
     lib.call("tb_router_groups", logits.data_ptr(), max(row, E), lib.ptr(bias), index.data_ptr(), weights.data_ptr(),
-             nt, E, k, groups, groups_use, group_top, scores == "softmax", bool(renorm), float(scale))
+             nt, E, k, groups, groups_use, group_top, scores == "softmax", bool(renorm), float(scale),
+             stream=lib.operator_stream())
