@@ -132,15 +132,39 @@ __global__ void __launch_bounds__(256) hd_pass_kernel(const HeadDecayArgs p) {
 }
 
 // ---- a segment's outputs --------------------------------------------------------------------------------------------
-// The rows of a segment, 4 x 4 a thread and tile of 64 columns, scaled, normed and gated where that is asked for.
+// The rows of a segment, 4 x 4 a thread and tile of 64 columns, scaled, normed and gated where that is asked for.  A row's gate is asked for
+// before the row ahead of it is stored (where registers hold both): behind a store that may change it a load waits for its turn.
 template <typename T, int TILES>
 __device__ __forceinline__ void hd_leave(const HeadDecayArgs& p, const HdSegment& s, int h, const F2 (&o)[TILES][4][2]) {
     const int vdim = p.vdim, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     T* out = static_cast<T*>(p.out) + (size_t)s.t0 * p.ldo + (size_t)h * vdim;
     const T* gate = static_cast<const T*>(p.gate) + (p.gate ? (size_t)s.t0 * p.ldgate + (size_t)h * vdim : 0);
+    constexpr bool AHEAD = TILES <= 2;
+    float z[2][TILES][4], nw[TILES][4];
+    auto ask = [&](int i) {
+        if (!p.gate || ty * 4 + i >= s.n) return;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int l = 0; l < 4; ++l) {
+                const int col = t * 64 + tx * 4 + l;
+                if (col < vdim) z[i & 1][t][l] = ldf(gate + (size_t)(ty * 4 + i) * p.ldgate + col);
+            }
+    };
+    if (p.gate)
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int l = 0; l < 4; ++l) {
+                const int col = t * 64 + tx * 4 + l;
+                if (col < vdim) nw[t][l] = p.norm[(size_t)h * vdim + col];
+            }
+    if (AHEAD) ask(0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int qi = ty * 4 + i;
+        if (!AHEAD) ask(i);
+        else if (i + 1 < 4) ask(i + 1);
         float sq = 0.f;
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
@@ -160,10 +184,7 @@ __device__ __forceinline__ void hd_leave(const HeadDecayArgs& p, const HdSegment
                 const int col = t * 64 + tx * 4 + l;
                 if (col >= vdim) continue;
                 float y = hd_of(o[t], i, l) * p.scale;
-                if (p.gate) {
-                    const float z = ldf(gate + (size_t)qi * p.ldgate + col);
-                    y = y * rs * p.norm[(size_t)h * vdim + col] * (z / (1.0f + expf(-z)));
-                }
+                if (p.gate) y = y * rs * nw[t][l] * (z[i & 1][t][l] / (1.0f + expf(-z[i & 1][t][l])));
                 stf(out + (size_t)qi * p.ldo + col, y);
             }
     }
@@ -200,7 +221,6 @@ __device__ __forceinline__ void hd_weigh(const float* p_s, const float* v_s, int
 template <typename T, int TILES>
 __device__ __forceinline__ void hd_rows(const HeadDecayArgs& p, const HdSegment& s, int h, const float* S, float* hd_sm, HdSum* c) {
     const int dim = p.dim, vdim = p.vdim;
-    hd_sums(p, h, s.t0, s.n, c);
     float* q_s = hd_sm;                          // [dim][HD_PAD]: q transposed, by token
     float* p_s = q_s + (size_t)dim * HD_PAD;     // [HD_SEG][HD_PAD]: weights transposed, [key][query]
     float* x_s = p_s + HD_SEG * HD_PAD;          // [64][HD_PAD]: keys transposed, states, values
@@ -216,9 +236,11 @@ __device__ __forceinline__ void hd_rows(const HeadDecayArgs& p, const HdSegment&
         hd_ask<HD_SEG>(x, [&](int r, int col) { return d0 + r < dim && c0 + col < vdim ? S[(size_t)(d0 + r) * vdim + c0 + col] : 0.f; });
     };
     auto ask_v = [&](int c0) { hd_ask<HD_SEG>(x, [&](int j, int col) { return j < s.n && c0 + col < vdim ? ldf(v + (size_t)j * p.ldv + c0 + col) : 0.f; }); };
+    ask_q(0);
+    hd_sums(p, h, s.t0, s.n, c);
     for (int d0 = 0; d0 < dim; d0 += 64) {
-        ask_q(d0);
         hd_put<HD_SEG>(x, [&](int i, int r, float y) { if (d0 + r < dim) q_s[(d0 + r) * HD_PAD + i] = y; });
+        if (d0 + 64 < dim) ask_q(d0 + 64);
     }
     // scores, rows = queries ty * 4 .., columns = keys tx * 4 ..
     F2 acc[4][2];
