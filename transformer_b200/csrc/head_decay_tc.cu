@@ -94,14 +94,15 @@ __device__ __forceinline__ void ht_load_tile(uint32_t dst, const CUtensorMap* ma
 }
 
 // y s(z) for two pairs, s(z) = z / (1 + e^-z).  The reciprocal on the multiply-add units, which have time where the exponential unit has
-// none: 0x7ef311c0 less the bits of x in [1, 2^116) is 1 / x within 5.1 %, and each Newton step r (2 - x r) squares that (6.7e-6 after two).
-// Below -80, where s is under 1e-33, z counts as -80 in the exponential.
+// none, by Newton and Raphson's steps r (2 - x r) from a start that is a subtraction of x's bits (the known piecewise linear approximation
+// by a float's exponent and fraction taken as one number): 0x7ef311c0 less the bits of x in [1, 2^116) is 1 / x within 5.1 %, and each step
+// squares that (6.7e-6 after two).  Below -80, where s lies between 0 and -1.5e-33, the reciprocal is 0 whatever the steps make of it, so that a
+// gate of the type's lowest value closes its channel; times -inf that is no number, as in the other kernels.
 __device__ __forceinline__ F2 ht_gated(F2 y, float z0, float z1) {
     F2 z, t, nx, r, m, c;
     z.f = make_float2(z0, z1);
     c.f = make_float2(-HT_LOG2E, -HT_LOG2E);
-    t.f = make_float2(fmaxf(z0, -80.f), fmaxf(z1, -80.f));
-    t = mul2(t, c);
+    t = mul2(z, c);
     t.f = make_float2(ht_ex2(t.f.x), ht_ex2(t.f.y));
     c.f = make_float2(-1.f, -1.f);
     nx = fma2(t, c, c);             // -(1 + e)
@@ -111,7 +112,8 @@ __device__ __forceinline__ F2 ht_gated(F2 y, float z0, float z1) {
     r = mul2(r, m);
     m = fma2(nx, r, c);
     r = mul2(r, m);
-    return mul2(mul2(y, z), r);
+    r.f = make_float2(z0 < -80.f ? 0.f : r.f.x, z1 < -80.f ? 0.f : r.f.y);
+    return mul2(y, mul2(z, r));
 }
 
 // The decays of a segment's tokens in blocks of 32: e_j = the sum behind token j to its block's end, l_j = up to and with token j from its
