@@ -118,16 +118,17 @@ __device__ __forceinline__ F2 ht_gated(F2 y, float z0, float z1) {
 
 // The decays of a segment's tokens in blocks of 32: e_j = the sum behind token j to its block's end, l_j = up to and with token j from its
 // block's start, and the sums before each block in 64 bits, so that no sum of few tokens is a difference of long ones.  The blocks that
-// make U leave them in scratch for those that make the outputs: a record of e [seg], l [seg], e^{e_j} [seg], the sums before the blocks, and a
+// make U leave them in scratch for those that make the outputs: a record of l [seg], e^{e_j} [seg], the sums before the blocks, and a
 // number for each of their worker warps that is not 0 if U has an entry that is no number there (which it has in a whole column where a value
-// of the segment is none: whatever it is multiplied with, the result is none).
+// of the segment is none: whatever it is multiplied with, the result is none).  A decay that is none is in e of the tokens before it, which
+// only tokens behind it may use: within a block the outputs take l, which has it from its token on.
 #define HT_BLOCKS (HT_MOST * HT_TILE / 32)
 struct alignas(16) HtSums {
     float e[HT_MOST * HT_TILE];
     double before[HT_BLOCKS + 2];
 };
-__host__ __device__ constexpr int ht_record_before(int seg) { return 3 * seg; }
-__host__ __device__ constexpr int ht_record_bad(int seg) { return 3 * seg + 2 * (HT_BLOCKS + 2); }
+__host__ __device__ constexpr int ht_record_before(int seg) { return 2 * seg; }
+__host__ __device__ constexpr int ht_record_bad(int seg) { return ht_record_before(seg) + 2 * (HT_BLOCKS + 2); }
 __host__ __device__ constexpr int ht_record(int seg) { return ht_record_bad(seg) + HT_WORKERS / 32; }
 #define HT_DECAYS (HT_MOST * HT_TILE / HT_WORKERS)      // tokens of a worker
 // This worker's tokens' decays, asked for ahead of ht_sums.
@@ -152,9 +153,8 @@ __device__ __forceinline__ void ht_sums(const HeadDecayArgs& p, int n, int tid, 
         s.e[i] = e;
         if (lane == 31) s.before[i >> 5] = (double)l;
         if (i < p.seg) {
-            record[i] = e;
-            record[p.seg + i] = l;
-            record[2 * p.seg + i] = ht_ex2(e * HT_LOG2E);
+            record[i] = l;
+            record[p.seg + i] = ht_ex2(e * HT_LOG2E);
         }
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -693,7 +693,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             const double* before = reinterpret_cast<const double*>(record + ht_record_before(p.seg));
             ok = ok && mbar_wait_warp(r_full(i), (i >> 1) & 1, a.error, 47);
             const bool look = __any_sync(0xffffffffu, lane < HT_WORKERS / 32 && record[ht_record_bad(p.seg) + (lane & 7)] != 0.f);
-            const float e_row = record[mine_at] * HT_LOG2E, l_row = record[p.seg + mine_at];
+            const float l_row = record[mine_at], l_row2 = l_row * HT_LOG2E;
             const double at_block = before[last * 4 + quad];
             ok = ok && mbar_wait_warp(o_start, i & 1, a.error, 47);
             tc_fence_after();
@@ -721,7 +721,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                         F2 f;
                         const float r = in ? ht_ex2((l_row + (float)(at_block - before[j * 4 + b + 1])) * HT_LOG2E) : 0.f;
                         f.f = make_float2(r, r);
-                        const float4* fk = reinterpret_cast<const float4*>(record + 2 * p.seg + j * HT_TILE + 32 * b);
+                        const float4* fk = reinterpret_cast<const float4*>(record + p.seg + j * HT_TILE + 32 * b);
 #pragma unroll
                         for (int c = 0; c < 8; ++c) {
                             const float4 y = fk[c];
@@ -737,14 +737,14 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                             w[2 * c + 1] = *reinterpret_cast<const uint32_t*>(&h1);
                         }
                     } else if (b == quad) {
-                        const float4* ek = reinterpret_cast<const float4*>(record + j * HT_TILE + 32 * b);
+                        const float4* lk = reinterpret_cast<const float4*>(record + j * HT_TILE + 32 * b);
 #pragma unroll
                         for (int c = 0; c < 8; ++c) {
-                            const float4 y = ek[c];
+                            const float4 y = lk[c];
                             const float z[4] = {y.x, y.y, y.z, y.w};
                             float o[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) o[e] = 4 * c + e <= lane ? v[4 * c + e] * ht_ex2(fmaf(z[e], HT_LOG2E, -e_row)) : 0.f;
+                            for (int e = 0; e < 4; ++e) o[e] = 4 * c + e <= lane ? v[4 * c + e] * ht_ex2(fmaf(z[e], -HT_LOG2E, l_row2)) : 0.f;
                             const __nv_bfloat162 h0 = __floats2bfloat162_rn(o[0], o[1]), h1 = __floats2bfloat162_rn(o[2], o[3]);
                             w[2 * c] = *reinterpret_cast<const uint32_t*>(&h0);
                             w[2 * c + 1] = *reinterpret_cast<const uint32_t*>(&h1);
