@@ -1,0 +1,56 @@
+"""The choice of experts where values meet that are near each other and values that are no numbers, against sorting in 64 bits by
+(is no number, larger first, lower index): every row's indices differ, and NaN comes behind -inf."""
+import math
+
+import pytest
+import torch
+
+from head_decay_plain import F32
+
+pytestmark = pytest.mark.gpu
+NAN, INF = float("nan"), float("inf")
+
+
+def _plain(x, k, scores, bias, groups=1, groups_use=1, group_top=1):
+    """(index, s of the chosen) for one row of floats."""
+    E, bias = len(x), [float(b) for b in bias]
+    if scores == "sigmoid":
+        s = [v if v != v else 1.0 / (1.0 + math.exp(-v)) if v > -700 else 0.0 for v in x]
+    else:
+        top = max(x, key=lambda v: -INF if v != v else v)
+        e = [NAN if v != v else 0.0 if v == -INF else math.exp(v - top) for v in x]
+        s = [v / sum(e) if sum(e) != 0 else 0.0 for v in e]
+    c = [a + b for a, b in zip(s, bias)]
+    number = lambda v: -INF if v != v else v
+    size = E // groups
+    worth = [number(sum(sorted((number(v) for v in c[j * size:(j + 1) * size]), reverse=True)[:group_top])) for j in range(groups)]
+    kept = sorted(range(groups), key=lambda j: (-worth[j], j))[:groups_use]
+    order = sorted((i for i in range(E) if i // size in kept), key=lambda i: (c[i] != c[i], -number(c[i]), i))[:k]
+    return order, [s[i] for i in order]
+
+
+def _hold(x, k, scores, bias, **how):
+    from transformer_b200.parts import choose_experts
+    x = torch.as_tensor(x, dtype=torch.float32)
+    bias = torch.as_tensor(bias, dtype=torch.float32)
+    idx = torch.full((x.shape[0], k), -7, dtype=torch.int32, device="cuda")
+    w = torch.full((x.shape[0], k), 7.0, device="cuda")
+    choose_experts(x.cuda(), idx, w, scores=scores, bias=bias.cuda(), **how)
+    idx, w = idx.cpu(), w.cpu().double()
+    for t, row in enumerate(x.tolist()):
+        order, s = _plain(row, k, scores, bias.tolist(), **how)
+        assert idx[t].tolist() == order, (row, bias.tolist(), how)
+        s = torch.tensor(s, dtype=torch.float64)
+        assert torch.equal(w[t].isnan(), s.isnan())
+        assert bool((((w[t] - s).abs() <= 64 * F32 * s.abs() + 1e-37) | s.isnan()).all())
+
+
+@pytest.mark.parametrize("k", [1, 2, 3, 4])
+def test_a_candidate_that_is_no_number(k):
+    """Saturated scores are near each other in float, 64 bits tell them apart; the NaN is among the k + 1 that are looked at."""
+    rows = [[20.0, 25.0, 0.0, NAN], [NAN, 25.0, 20.0, 0.0], [20.0, NAN, 0.0, 25.0], [25.0, 20.0, NAN, NAN], [NAN, NAN, NAN, 20.0],
+            [20.0, 25.0, 60.0, NAN], [-INF, 25.0, 20.0, NAN], [20.0, 20.0, NAN, 25.0], [NAN, NAN, NAN, NAN]]
+    _hold(rows, k, "sigmoid", [0.0] * 4)
+    _hold(rows, k, "sigmoid", [0.0, 0.0, 0.0, NAN])
+    _hold(rows, k, "sigmoid", [0.0, 0.0, -INF, 0.0])
+    _hold(rows, k, "sigmoid", [1e-9, 0.0, 0.0, 1e-9])

@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_groups_kernel(const __gr
             } else if ((closes & ((1u << p.k) - 1u)) && p.softmax) {
                 again = true;       // a sum over all experts is wanted
             } else if (closes & ((1u << p.k) - 1u)) {
-                // the candidates in 64 bits, a lane each, to their places by counting
+                // the candidates in 64 bits, a lane each, to their places by counting; NaN, which compares with nothing, behind all numbers
                 const double d = have && lane <= p.k ? 1.0 / (1.0 + exp(-(double)mine_x)) + (double)b : 0.0;
                 const bool counts = have && lane <= p.k;
                 int place = 0;
@@ -342,7 +342,8 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_groups_kernel(const __gr
                     const double od = __shfl_sync(0xffffffffu, d, j);
                     const int oe = __shfl_sync(0xffffffffu, mine, j);
                     const int there = __shfl_sync(0xffffffffu, (int)counts, j);
-                    place += there && (od > d || (od == d && oe < mine));
+                    const bool on = od != od, dn = d != d;
+                    place += there && (od > d || (dn && !on) || ((od == d || (on && dn)) && oe < mine));
                 }
                 const int was = mine;
                 for (int j = 0; j <= p.k; ++j) {
