@@ -54,3 +54,26 @@ def test_a_candidate_that_is_no_number(k):
     _hold(rows, k, "sigmoid", [0.0, 0.0, 0.0, NAN])
     _hold(rows, k, "sigmoid", [0.0, 0.0, -INF, 0.0])
     _hold(rows, k, "sigmoid", [1e-9, 0.0, 0.0, 1e-9])
+
+
+@pytest.mark.parametrize("E,k,groups,groups_use", [(12, 5, 1, 1), (12, 8, 1, 1), (40, 9, 4, 1), (40, 10, 4, 1), (64, 6, 8, 3), (96, 24, 4, 1),
+                                                   (256, 8, 8, 4), (300, 30, 1, 1), (600, 9, 6, 2)])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_rows_of_near_values_and_none(E, k, groups, groups_use, scores):
+    gen = torch.Generator().manual_seed(E + k)
+    pick = lambda values, share: torch.where(torch.rand(30, E, generator=gen) < share, torch.tensor(values)[torch.randint(0, len(values), (30, E), generator=gen)], 0.0)
+    near = torch.full((30, E), 1.25).view(torch.int32) + torch.randint(0, 5, (30, E), generator=gen, dtype=torch.int32)
+    x = near.view(torch.float32) + pick([20.0, 25.0, 60.0, -3.0] if scores == "sigmoid" else [-3.0, 0.5], 0.5)
+    if scores == "sigmoid":             # one NaN of a softmax is all of its row's, which the last test looks at
+        x = x + pick([NAN, -INF], 0.3)
+    masks = torch.zeros(E)
+    masks[torch.randperm(E, generator=gen)[: E // 4]] = -INF
+    nans = masks.clone()
+    nans[torch.randperm(E, generator=gen)[: E // 8 + 1]] = NAN
+    for bias in (torch.zeros(E), masks, nans, torch.randint(0, 2, (E,), generator=gen) * 1e-8):
+        for top in (1, 2):
+            _hold(x, k, scores, bias, groups=groups, groups_use=groups_use, group_top=top)
+
+
+def test_one_that_is_none_is_all_of_a_softmax():
+    _hold([[1.0, NAN, 2.0, 3.0], [NAN, -INF, -INF, -INF]], 3, "softmax", [0.0, 0.0, 1.0, -INF])

@@ -15,7 +15,7 @@
 // 2,039 tokens, 4 of 60, 4 us; 8 tokens 4 us.
 #include "common.cuh"
 
-#define RG_MAX_E 1024
+#define RG_MAX_E 1024           // a power of two
 #define RG_MAX_K 30
 #define RG_MAX_GROUPS 32
 #define RG_WARPS 8
@@ -65,7 +65,7 @@ __device__ __noinline__ int rg_choose64(const RouterGroupArgs& p, const float* r
     const double lowest = -INFINITY;
     const int size = p.E / p.groups;
     double c[PER];
-    unsigned open = 0u;             // which of the lane's may be chosen
+    unsigned open = 0u, none = 0u;  // which of the lane's may be chosen, and which are NaN
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int e = lane * PER + i;
@@ -86,7 +86,10 @@ __device__ __noinline__ int rg_choose64(const RouterGroupArgs& p, const float* r
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         if (p.bias && (open >> i & 1u)) c[i] += (double)p.bias[lane * PER + i];
-        if (c[i] != c[i]) c[i] = lowest;
+        if (c[i] != c[i]) {
+            c[i] = lowest;
+            none |= 1u << i;
+        }
     }
     if (p.groups > 1) {
         double worth = lowest;      // of group `lane`
@@ -124,13 +127,15 @@ __device__ __noinline__ int rg_choose64(const RouterGroupArgs& p, const float* r
     int mine = 0;
     for (int j = 0; j < p.k; ++j) {
         double best = lowest;
-        int at = 0x7fffffff;
+        int at = 0x7fffffff;        // among equals the least; NaN stands behind -inf by a number above all experts'
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if ((open >> i & 1u) && (at == 0x7fffffff || c[i] > best)) {
+        for (int i = 0; i < PER; ++i) {
+            const int e = lane * PER + i + (none >> i & 1u ? RG_MAX_E : 0);
+            if ((open >> i & 1u) && (at == 0x7fffffff || c[i] > best || (c[i] == best && e < at))) {
                 best = c[i];
-                at = lane * PER + i;
+                at = e;
             }
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const double ov = __shfl_xor_sync(0xffffffffu, best, o);
@@ -140,6 +145,7 @@ __device__ __noinline__ int rg_choose64(const RouterGroupArgs& p, const float* r
                 at = oi;
             }
         }
+        at &= RG_MAX_E - 1;
         if (at / PER == lane) open &= ~(1u << (at - lane * PER));
         if (lane == j) mine = at;
     }
