@@ -1,5 +1,6 @@
 """The choice of experts where values meet that are near each other and values that are no numbers, against sorting in 64 bits by
-(is no number, larger first, lower index): every row's indices differ, and NaN comes behind -inf."""
+(is no number, larger first, lower index): every row's indices differ, NaN comes behind -inf, and a group's worth that is no number
+counts as -inf."""
 import math
 
 import pytest
@@ -77,3 +78,16 @@ def test_rows_of_near_values_and_none(E, k, groups, groups_use, scores):
 
 def test_one_that_is_none_is_all_of_a_softmax():
     _hold([[1.0, NAN, 2.0, 3.0], [NAN, -INF, -INF, -INF]], 3, "softmax", [0.0, 0.0, 1.0, -INF])
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_a_worth_of_infinity_less_infinity(scores):
+    """Groups of two, one of them with a bias of both infinities: no worth at all, so the others are used."""
+    x = torch.randn(20, 8, generator=torch.Generator().manual_seed(3))
+    for at in range(0, 8, 2):
+        bias = torch.zeros(8)
+        bias[at], bias[at + 1] = INF, -INF
+        for use, k in ((1, 2), (2, 4), (3, 6)):
+            _hold(x, k, scores, bias, groups=4, groups_use=use, group_top=2)
+        bias[(at + 2) % 8], bias[(at + 3) % 8] = -INF, INF
+        _hold(x, 4, scores, bias, groups=4, groups_use=2, group_top=2)

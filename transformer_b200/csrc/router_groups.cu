@@ -5,7 +5,8 @@
 //   the k largest c of those are chosen, in descending order;  w = s of the chosen, / their sum with `renorm`, times `scale`
 //
 // Equal c, or groups of equal worth, go to the lower index.  An expert with logit -inf has s = 0 (in a row of nothing else too); NaN ranks
-// below -inf, so the k indices of a row always differ; chosen scores that are all 0 stay 0 when they are renormalized.
+// below -inf, and in a group's worth it counts as -inf, as inf - inf does, so the k indices of a row always differ; chosen scores that are
+// all 0 stay 0 when they are renormalized.
 //
 // A warp per token, a lane the PER neighbouring experts from lane * PER on: the lowest lane among equals has the lowest index, so
 // a choice is one redux over order-preserving keys, a ballot and a shuffle.  Without a bias c and x have the same order, and the
@@ -110,6 +111,7 @@ __device__ __noinline__ int rg_choose64(const RouterGroupArgs& p, const float* r
             }
             if (lane == g) worth = p.group_top == 2 && size > 1 ? a + b : a;
         }
+        if (worth != worth) worth = lowest;
         int place = 0;
         for (int g = 0; g < p.groups; ++g) {
             const double other = __shfl_sync(0xffffffffu, worth, g);
@@ -235,7 +237,8 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_groups_kernel(const __gr
             b = fmaxf(fminf(a, oa), fmaxf(b, ob));
             a = fmaxf(a, oa);
         }
-        const float worth = p.group_top == 2 && size > 1 ? a + b : a;
+        float worth = p.group_top == 2 && size > 1 ? a + b : a;
+        if (worth != worth) worth = -INFINITY;      // a bias of inf and one of -inf
         int place = 0;
         for (int j = 0; j < p.groups; ++j) {
             const float other = __shfl_sync(0xffffffffu, worth, j * L);
