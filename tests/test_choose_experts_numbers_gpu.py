@@ -91,3 +91,14 @@ def test_a_worth_of_infinity_less_infinity(scores):
             _hold(x, k, scores, bias, groups=4, groups_use=use, group_top=2)
         bias[(at + 2) % 8], bias[(at + 3) % 8] = -INF, INF
         _hold(x, 4, scores, bias, groups=4, groups_use=2, group_top=2)
+
+
+def test_the_most_tokens():
+    """2^31 - 1 rows of one expert (26 GB): as many blocks as that is."""
+    from transformer_b200.parts import choose_experts
+    n = 2 ** 31 - 1
+    x, idx, w = torch.zeros((n, 1), device="cuda"), torch.full((n, 1), 7, dtype=torch.int32, device="cuda"), torch.zeros((n, 1), device="cuda")
+    choose_experts(x, idx, w)
+    assert not bool(idx.any()) and bool((w == 1).all())
+    del x, idx, w
+    torch.cuda.empty_cache()

@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(RG_WARPS * 32) router_groups_kernel(const __gr
 template <int PER>
 static void router_groups_launch(const RouterGroupArgs& p, cudaStream_t s) {
     const size_t smem = p.groups > 1 ? (size_t)RG_WARPS * (p.E + p.E / 32 + 1) * sizeof(float) : 0;
-    TB_LAUNCH((router_groups_kernel<PER>), (p.nt + RG_WARPS - 1) / RG_WARPS, RG_WARPS * 32, smem, s, p);
+    TB_LAUNCH((router_groups_kernel<PER>), (p.nt - 1) / RG_WARPS + 1, RG_WARPS * 32, smem, s, p);
 }
 
 extern "C" int tb_router_groups(const float* logits, long long ld, const float* bias, int* idx, float* w, int nt, int E, int k,
