@@ -536,8 +536,9 @@ static int hd_prompt_launch(HeadDecayArgs p, int heads, cudaStream_t s) {
         TB_LAUNCH((hd_short_kernel<T>), dim3(p.B, p.H), 256, smem, s, p);
         return tb_last_error();
     }
-    if (p.max_segs < p.nt / p.seg + p.B) return TB_ERR_ARG;
-    p.max_segs = p.nt / p.seg + p.B;
+    const long long segs = hd_segments(p.nt, p.B, p.seg);
+    if (p.max_segs < segs) return TB_ERR_ARG;
+    p.max_segs = (int)segs;
     const int size = p.dim * p.vdim, tiles = ((p.dim + 63) / 64) * ((p.vdim + 63) / 64);
     p.seg_g = p.work + (size_t)heads * p.max_segs * size;
     for (p.h0 = 0; p.h0 < p.H; p.h0 += heads) {
@@ -569,8 +570,11 @@ static int hd_step_launch(const HeadDecayArgs& p, cudaStream_t s) {
 }
 
 extern "C" {
-// 0: one kernel does all, no scratch is wanted.
-int tb_head_decay_segments(int nt, int B, int dim, int vdim) { return hd_is_short(nt, dim, vdim) ? 0 : nt / HD_SEG + B; }
+// 0: one kernel does all, no scratch is wanted.  -1: more segments than 32 bits count.
+int tb_head_decay_segments(int nt, int B, int dim, int vdim) {
+    const long long segs = hd_is_short(nt, dim, vdim) ? 0 : hd_segments(nt, B, HD_SEG);
+    return segs > 0x7fffffffLL ? -1 : (int)segs;
+}
 
 int tb_head_decay_rates(const float* a, const float* rate, const float* bias, float* g, int nt, int H, cudaStream_t s) {
     if (nt < 0 || H <= 0 || (long long)nt * H > 0x7fffffffLL - 256) return TB_ERR_ARG;

@@ -101,6 +101,9 @@ __device__ __forceinline__ void hd_sums(const HeadDecayArgs& p, int h, int t0, i
     }
 }
 
+// Segments of B sequences of nt tokens in all, at most.
+static inline long long hd_segments(int nt, int B, int seg) { return (long long)nt / seg + B; }
+
 // What every launcher asks of its sizes.
 static inline int hd_check(const HeadDecayArgs& p) {
     if (p.nt < 0 || p.B < 0 || p.H <= 0 || p.G <= 0 || p.H % p.G || p.dim <= 0 || p.vdim <= 0 || p.n_slots < 0 ||

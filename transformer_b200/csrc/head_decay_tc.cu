@@ -884,7 +884,7 @@ static void ht_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtens
 
 // Floats of scratch a head for segments of `tiles` tiles: U, S_0 (bfloat16), the tokens' decays and the segments'.
 static long long ht_work(int nt, int B, int dim, int vdim, int tiles) {
-    const long long segs = nt / (tiles * HT_TILE) + B, size = (long long)dim * vdim;
+    const long long segs = hd_segments(nt, B, tiles * HT_TILE), size = (long long)dim * vdim;
     return (segs * (size + size / 2 + ht_record(tiles * HT_TILE)) + segs + 3) / 4 * 4;
 }
 
@@ -913,8 +913,9 @@ int tb_head_decay_tc_bf16(const void* q, const void* k, const void* v, const voi
           (uintptr_t)norm) & 15))
         return TB_ERR_UNSUPPORTED;
     if (B == 0) return 0;
-    p.max_segs = nt / p.seg + B;
-    if ((long long)p.max_segs * tiles > 0x7fffffffLL) return TB_ERR_UNSUPPORTED;
+    const long long segs = hd_segments(nt, B, p.seg);
+    if (segs * tiles > 0x7fffffffLL) return TB_ERR_UNSUPPORTED;
+    p.max_segs = (int)segs;
     if (heads > H) heads = H;
     const size_t size = (size_t)dim * vdim, all = (size_t)heads * p.max_segs;
     a.starts = reinterpret_cast<__nv_bfloat16*>(work + all * size);

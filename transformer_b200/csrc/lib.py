@@ -524,7 +524,7 @@ def split_delta_record_size(dim: int) -> int:
 @functools.lru_cache(maxsize=4096)
 def head_decay_segments(tokens: int, sequences: int, dim: int, vdim: int) -> int:
     """Segments that a step's tokens are cut into at most, for the linear attention with one decay a head; 0: so few tokens and small
-    heads that one kernel does all without scratch."""
+    heads that one kernel does all without scratch; -1: more than 32 bits count."""
     return library().tb_head_decay_segments(tokens, sequences, dim, vdim)
 
 

@@ -80,6 +80,8 @@ def _checked(q, k, v, log_decay, state, slots, out, norm, gate, new_state, seq_s
             raise ValueError(f"new_state has {new_state.shape[0]} slots, state {n_slots}")
     if max(nt, n_slots, slots.numel()) > MOST_ROWS:
         raise ValueError(f"{nt} tokens, {slots.numel()} sequences, {n_slots} slots: at most {MOST_ROWS} of each")
+    if seq_start is not None and lib.head_decay_segments(nt, slots.numel(), dim, vdim) < 0:
+        raise ValueError(f"{nt} tokens in {slots.numel()} sequences may be more than {MOST_ROWS} segments")
     if slots.dtype is not torch.int32 or slots.dim() != 1 or not slots.is_contiguous():
         raise ValueError("slots must be a contiguous int32 tensor")
     if (norm is None) != (gate is None):
