@@ -16,6 +16,11 @@ def test_counts_in_more_than_32_bits():
     assert lib.library().tb_head_decay_segments(MOST, MOST, 64, 64) < 0
 
 
+def test_scratch_in_more_than_32_bits():
+    few, many = lib.head_decay_tc_work(MOST, 1, 64, 64), lib.head_decay_tc_work(MOST, MOST, 64, 64)
+    assert 0 < few < many and many > (MOST + MOST // 256) * 64 * 64
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("nt,B", [(MOST, MOST), (64 * 2 ** 20, MOST), (MOST, MOST - MOST // 64 + 1)])
 def test_more_segments_than_32_bits_count(nt, B, dtype):

@@ -27,7 +27,9 @@
 
 #define HT_TILE 128
 #define HT_HALF 64              // rows of a TMA box, and keys that the update takes together
-#define HT_MOST 2               // most tiles of a segment
+#define HT_TILES 2              // tiles of a segment: with 1 and 2, 2,048 tokens of 32 heads 60 and 51 us, 11,875 in 11 sequences 299 and 241 (twice
+                                // the states' way through memory); 4 left the SMs with few long blocks (61 and 268)
+#define HT_SEG (HT_TILES * HT_TILE)
 #define HT_WORKERS 256          // eight warps: two for each 32 lanes of tensor memory, half of the columns each
 #define HT_THREADS (64 + HT_WORKERS)
 #define HT_LOG2E 1.4426950408889634f
@@ -35,9 +37,8 @@
 struct HdTcArgs {
     HeadDecayArgs p;
     __nv_bfloat16* starts;          // [heads of a portion][max_segs][dim][vdim]
-    float* sums;                    // [heads of a portion][max_segs][ht_record(seg)]
+    float* sums;                    // [heads of a portion][max_segs][HT_RECORD]
     int* error;
-    int tiles;                      // of a segment: seg / HT_TILE
     int heads_u, heads_r;           // heads that a block goes through, one after the other
 };
 
@@ -122,15 +123,16 @@ __device__ __forceinline__ F2 ht_gated(F2 y, float z0, float z1) {
 // number for each of their worker warps that is not 0 if U has an entry that is no number there (which it has in a whole column where a value
 // of the segment is none: whatever it is multiplied with, the result is none).  A decay that is none is in e of the tokens before it, which
 // only tokens behind it may use: within a block the outputs take l, which has it from its token on.
-#define HT_BLOCKS (HT_MOST * HT_TILE / 32)
+#define HT_BLOCKS (HT_SEG / 32)
 struct alignas(16) HtSums {
-    float e[HT_MOST * HT_TILE];
+    float e[HT_SEG];
     double before[HT_BLOCKS + 2];
 };
-__host__ __device__ constexpr int ht_record_before(int seg) { return 2 * seg; }
-__host__ __device__ constexpr int ht_record_bad(int seg) { return ht_record_before(seg) + 2 * (HT_BLOCKS + 2); }
-__host__ __device__ constexpr int ht_record(int seg) { return ht_record_bad(seg) + HT_WORKERS / 32; }
-#define HT_DECAYS (HT_MOST * HT_TILE / HT_WORKERS)      // tokens of a worker
+#define HT_RECORD_BEFORE (2 * HT_SEG)
+#define HT_RECORD_BAD (HT_RECORD_BEFORE + 2 * (HT_BLOCKS + 2))
+#define HT_RECORD (HT_RECORD_BAD + HT_WORKERS / 32)
+#define HT_DECAYS (HT_SEG / HT_WORKERS)         // tokens of a worker
+static_assert(HT_SEG % HT_WORKERS == 0 && HT_BLOCKS < 32, "a worker's tokens, and the blocks' sums in one warp");
 // This worker's tokens' decays, asked for ahead of ht_sums.
 __device__ __forceinline__ void ht_decays(const HeadDecayArgs& p, int h, int t0, int n, int tid, float (&x)[HT_DECAYS]) {
 #pragma unroll
@@ -152,10 +154,8 @@ __device__ __forceinline__ void ht_sums(const HeadDecayArgs& p, int n, int tid, 
         }
         s.e[i] = e;
         if (lane == 31) s.before[i >> 5] = (double)l;
-        if (i < p.seg) {
-            record[i] = l;
-            record[p.seg + i] = ht_ex2(e * HT_LOG2E);
-        }
+        record[i] = l;
+        record[HT_SEG + i] = ht_ex2(e * HT_LOG2E);
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
     if (tid < 32) {         // the blocks' sums, to those before each
@@ -168,7 +168,7 @@ __device__ __forceinline__ void ht_sums(const HeadDecayArgs& p, int n, int tid, 
         const double before = __shfl_up_sync(0xffffffffu, v, 1);
         if (lane <= HT_BLOCKS) {
             s.before[lane] = lane ? before : 0.0;
-            reinterpret_cast<double*>(record + ht_record_before(p.seg))[lane] = lane ? before : 0.0;
+            reinterpret_cast<double*>(record + HT_RECORD_BEFORE)[lane] = lane ? before : 0.0;
         }
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -304,7 +304,7 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 }
             }
             const bool some = __any_sync(0xffffffffu, !(bad == 0.f));
-            if (lane == 0) a.sums[at * ht_record(p.seg) + ht_record_bad(p.seg) + (tid >> 5)] = some ? 1.f : 0.f;
+            if (lane == 0) a.sums[at * HT_RECORD + HT_RECORD_BAD + (tid >> 5)] = some ? 1.f : 0.f;
             tc_fence_before();
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(u_empty(i & 1)) : "memory");
@@ -312,7 +312,7 @@ hd_update_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         for (int i = 0, it = 0; i < heads; ++i) {
             HtSums& sum = sums[i & 1];
             const size_t at = (size_t)(at0 + i) * p.max_segs + blockIdx.x;
-            ht_sums(p, s.n, tid, x, sum, a.sums + at * ht_record(p.seg));
+            ht_sums(p, s.n, tid, x, sum, a.sums + at * HT_RECORD);
             if (i + 1 < heads) ht_decays(p, p.h0 + at0 + i + 1, s.t0, s.n, tid, x);
             const double end = sum.before[(s.n + 31) / 32];
             for (int j = 0; j < tiles; ++j, ++it) {
@@ -389,8 +389,8 @@ __global__ void __launch_bounds__(256) hd_pass_tc_kernel(const HdTcArgs a) {
     };
     float S[4];
     once(p.state + (size_t)slot * p.pitch + (size_t)h * size + e, S);
-    const int segs = (n + p.seg - 1) / p.seg;
-    const size_t first = (size_t)blockIdx.y * p.max_segs + t0 / p.seg + b;
+    const int segs = (n + HT_SEG - 1) / HT_SEG;
+    const size_t first = (size_t)blockIdx.y * p.max_segs + t0 / HT_SEG + b;
     const float* __restrict__ w = p.work + first * size + ((size_t)(c >> 2) * p.dim + r) * 4;
     const float* __restrict__ gs = p.seg_g + first;
     __nv_bfloat16* __restrict__ st = a.starts + first * size + e;
@@ -465,7 +465,7 @@ __device__ __noinline__ void ht_unclear(const __nv_bfloat16* seen, long long ldv
 }
 
 struct alignas(16) HtRowsShared {
-    float record[2][ht_record(HT_MOST * HT_TILE)];          // of the head, by its parity
+    float record[2][HT_RECORD];          // of the head, by its parity
     float norm[2][256];
     float squares[2][HT_TILE];
 };
@@ -500,7 +500,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 14);
     volatile uint32_t* cleared = reinterpret_cast<volatile uint32_t*>(bars + 15);       // by the head's parity
     const int warp = warp_number(), lane = threadIdx.x & 31;
-    const int x = blockIdx.x / a.tiles, at0 = blockIdx.y * a.heads_r, heads = min(a.heads_r, p.heads - at0);
+    const int x = blockIdx.x / HT_TILES, at0 = blockIdx.y * a.heads_r, heads = min(a.heads_r, p.heads - at0);
     const uint32_t bar0 = smem_u32(bars), q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 16, v_full = bar0 + 24, v_empty = bar0 + 32,
                    s_full = bar0 + 40, p_ready = bar0 + 48, o_start = bar0 + 56, o_done = bar0 + 64, g_full = bar0 + 72, x_free = bar0 + 80;
     auto r_full = [&](int i) { return bar0 + 88 + 8u * (i & 1); };
@@ -528,7 +528,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     __syncwarp();
     if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
     const HdSegment s = hd_find(p, x);
-    const int last = blockIdx.x - x * a.tiles;              // this block's tile of its segment
+    const int last = blockIdx.x - x * HT_TILES;              // this block's tile of its segment
     const int q0 = s.t0 + last * HT_TILE, nq = min(HT_TILE, s.n - last * HT_TILE);      // nq <= 0: no such tile
     const int n_k = last + 1, n_v = last + 2;               // phases of a head: tiles of keys; S_0 and tiles of values
     auto kv_of = [&](int i) { return (p.h0 + at0 + i) / (p.H / p.G); };
@@ -547,9 +547,9 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ht_load_tile<KB>(sy(i), &map_k, k_full, kv_of(i), s.t0 + j * HT_TILE);
     };
     auto load_record = [&](int i) {
-        const uint32_t bytes = ht_record(p.seg) * 4, nb = p.gate ? p.vdim * 4 : 0;
+        const uint32_t bytes = HT_RECORD * 4, nb = p.gate ? p.vdim * 4 : 0;
         mbar_expect_tx(r_full(i), bytes + nb);
-        bulk_load(smem_u32(sh.record[i & 1]), a.sums + ((size_t)(at0 + i) * p.max_segs + x) * ht_record(p.seg), bytes, r_full(i));
+        bulk_load(smem_u32(sh.record[i & 1]), a.sums + ((size_t)(at0 + i) * p.max_segs + x) * HT_RECORD, bytes, r_full(i));
         if (nb) bulk_load(smem_u32(sh.norm[i & 1]), p.norm + (size_t)(p.h0 + at0 + i) * p.vdim, nb, r_full(i));
     };
     // the first copies do not wait for the other warps: this one has made their barriers
@@ -690,9 +690,9 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         for (int i = 0; i < heads; ++i) {
             const uint32_t to = tmem_o(i) + lane_sel, ts = tmem_s(i) + lane_sel;
             const float* record = sh.record[i & 1];
-            const double* before = reinterpret_cast<const double*>(record + ht_record_before(p.seg));
+            const double* before = reinterpret_cast<const double*>(record + HT_RECORD_BEFORE);
             ok = ok && mbar_wait_warp(r_full(i), (i >> 1) & 1, a.error, 47);
-            const bool look = __any_sync(0xffffffffu, lane < HT_WORKERS / 32 && record[ht_record_bad(p.seg) + (lane & 7)] != 0.f);
+            const bool look = __any_sync(0xffffffffu, lane < HT_WORKERS / 32 && record[HT_RECORD_BAD + (lane & 7)] != 0.f);
             const float l_row = record[mine_at], l_row2 = l_row * HT_LOG2E;
             const double at_block = before[last * 4 + quad];
             ok = ok && mbar_wait_warp(o_start, i & 1, a.error, 47);
@@ -721,7 +721,7 @@ hd_rows_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                         F2 f;
                         const float r = in ? ht_ex2((l_row + (float)(at_block - before[j * 4 + b + 1])) * HT_LOG2E) : 0.f;
                         f.f = make_float2(r, r);
-                        const float4* fk = reinterpret_cast<const float4*>(record + p.seg + j * HT_TILE + 32 * b);
+                        const float4* fk = reinterpret_cast<const float4*>(record + HT_SEG + j * HT_TILE + 32 * b);
 #pragma unroll
                         for (int c = 0; c < 8; ++c) {
                             const float4 y = fk[c];
@@ -879,48 +879,43 @@ static void ht_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtens
     const dim3 grid(p.B, p.heads, (p.dim / 8 * ((p.vdim + 15) / 16) + 7) / 8);
     if ((long long)grid.x * grid.y * grid.z <= 148 * 8) TB_LAUNCH((hd_pass_tc_kernel<8>), grid, 256, 0, s, a);
     else TB_LAUNCH((hd_pass_tc_kernel<4>), grid, 256, 0, s, a);
-    if (p.nt) TB_LAUNCH((hd_rows_tc_kernel<KB, VB>), dim3(p.max_segs * a.tiles, (p.heads + a.heads_r - 1) / a.heads_r), HT_THREADS, smem_r, s, mq, mk, mv, ms, mg, mo, a);
-}
-
-// Floats of scratch a head for segments of `tiles` tiles: U, S_0 (bfloat16), the tokens' decays and the segments'.
-static long long ht_work(int nt, int B, int dim, int vdim, int tiles) {
-    const long long segs = hd_segments(nt, B, tiles * HT_TILE), size = (long long)dim * vdim;
-    return (segs * (size + size / 2 + ht_record(tiles * HT_TILE)) + segs + 3) / 4 * 4;
+    if (p.nt) TB_LAUNCH((hd_rows_tc_kernel<KB, VB>), dim3(p.max_segs * HT_TILES, (p.heads + a.heads_r - 1) / a.heads_r), HT_THREADS, smem_r, s, mq, mk, mv, ms, mg, mo, a);
 }
 
 extern "C" {
-// 0: these kernels do not take such heads.
-long long tb_head_decay_tc_work(int nt, int B, int dim, int vdim, int tiles) {
-    if (dim <= 0 || vdim <= 0 || dim % 8 || vdim % 8 || dim > 128 || vdim > 256 || tiles < 1 || tiles > HT_MOST) return 0;
-    return ht_work(nt, B, dim, vdim, tiles);
+// Floats of scratch a head: U, S_0 (bfloat16), the tokens' decays and the segments'.  0: these kernels do not take such heads.
+long long tb_head_decay_tc_work(int nt, int B, int dim, int vdim) {
+    if (dim <= 0 || vdim <= 0 || dim % 8 || vdim % 8 || dim > 128 || vdim > 256) return 0;
+    const long long segs = hd_segments(nt, B, HT_SEG), size = (long long)dim * vdim;
+    return (segs * (size + size / 2 + HT_RECORD) + segs + 3) / 4 * 4;
 }
 
 int tb_head_decay_tc_bf16(const void* q, const void* k, const void* v, const void* gate, long long ldq, long long ldk, long long ldv,
                           long long ldgate, const float* g, long long g_stride, const float* norm, const float* state, float* new_state,
                           long long pitch, long long new_pitch, void* out, long long ldo, const int* seq_start, const int* slots,
-                          float* work, int tiles, int heads, int nt, int B, int H, int G, int dim, int vdim, int n_slots, float scale,
+                          float* work, int heads, int nt, int B, int H, int G, int dim, int vdim, int n_slots, float scale,
                           float eps, cudaStream_t s) {
     HdTcArgs a{HeadDecayArgs{q, k, v, gate, g, norm, state, new_state, out, seq_start, slots, work, nullptr, ldq, ldk, ldv, ldgate, ldo,
-                             pitch, new_pitch, g_stride, nt, B, H, G, dim, vdim, n_slots, 0, tiles * HT_TILE, 0, H, scale, eps},
-               nullptr, nullptr, nullptr, tiles, 1, 1};
+                             pitch, new_pitch, g_stride, nt, B, H, G, dim, vdim, n_slots, 0, HT_SEG, 0, H, scale, eps},
+               nullptr, nullptr, nullptr, 1, 1};
     HeadDecayArgs& p = a.p;
     const int rc = hd_check(p);
     if (rc) return rc;
     if (heads <= 0 || ((uintptr_t)work & 15)) return TB_ERR_ARG;
-    if (!tb_head_decay_tc_work(nt, B, dim, vdim, tiles)) return TB_ERR_UNSUPPORTED;
+    if (!tb_head_decay_tc_work(nt, B, dim, vdim)) return TB_ERR_UNSUPPORTED;
     if (ldq % 8 || ldk % 8 || ldv % 8 || ldo % 8 || ldgate % 8 || pitch % 4 || new_pitch % 4 ||
         (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)gate | (uintptr_t)out | (uintptr_t)state | (uintptr_t)new_state |
           (uintptr_t)norm) & 15))
         return TB_ERR_UNSUPPORTED;
     if (B == 0) return 0;
     const long long segs = hd_segments(nt, B, p.seg);
-    if (segs * tiles > 0x7fffffffLL) return TB_ERR_UNSUPPORTED;
+    if (segs * HT_TILES > 0x7fffffffLL) return TB_ERR_UNSUPPORTED;
     p.max_segs = (int)segs;
     if (heads > H) heads = H;
     const size_t size = (size_t)dim * vdim, all = (size_t)heads * p.max_segs;
     a.starts = reinterpret_cast<__nv_bfloat16*>(work + all * size);
     a.sums = work + all * size + all * (size / 2);
-    p.seg_g = a.sums + all * ht_record(p.seg);
+    p.seg_g = a.sums + all * HT_RECORD;
     a.error = tc_error_ptr();
     if (!a.error) return tb_last_error();
     // Heads a block: the next one's copies run ahead, but longer blocks leave the SMs less evenly.  Up to four, where three rounds of blocks
@@ -930,7 +925,7 @@ int tb_head_decay_tc_bf16(const void* q, const void* k, const void* v, const voi
     const long long places = 2 * 148;
     auto per_block = [&](long long blocks) { return (int)std::max(1LL, std::min({4LL, (long long)heads, blocks * heads / (3 * places)})); };
     a.heads_u = per_block(p.max_segs);
-    a.heads_r = per_block((long long)p.max_segs * tiles);
+    a.heads_r = per_block((long long)p.max_segs * HT_TILES);
     const int kb = (dim + 63) / 64, vb = vdim <= 64 ? 1 : vdim <= 128 ? 2 : 4;
     CUtensorMap mq, mk, mv, ms, mo, mg = {};
     const int rows = nt > 0 ? nt : 1;

@@ -115,7 +115,7 @@ _SIGNATURES: Dict[str, str] = {
     "tb_post_add_layernorm_router_bf16": "pppppippfipppfipiippppiii",
     "tb_head_decay_f32": "ppppllllplpppllplpppiiiiiiiiiff", "tb_head_decay_bf16": "ppppllllplpppllplpppiiiiiiiiiff",
     "tb_head_decay_step_f32": "ppppllllplpppllplpiiiiiiff", "tb_head_decay_step_bf16": "ppppllllplpppllplpiiiiiiff",
-    "tb_head_decay_tc_bf16": "ppppllllplpppllplpppiiiiiiiiiff",
+    "tb_head_decay_tc_bf16": "ppppllllplpppllplpppiiiiiiiiff",
     "tb_head_decay_rates": "ppppii",
     "tb_router_groups": "plpppiiiiiiiif",
 }
@@ -171,7 +171,7 @@ def library() -> ctypes.CDLL:
                 fn = getattr(lib, name)
                 fn.argtypes = [_CODES[c] for c in codes]
                 fn.restype = _I
-            lib.tb_head_decay_tc_work.argtypes = [_I] * 5
+            lib.tb_head_decay_tc_work.argtypes = [_I] * 4
             lib.tb_head_decay_tc_work.restype = _L
             lib.tb_tape_index.argtypes = [ctypes.c_char_p]
             lib.tb_tape_index.restype = _I
@@ -529,10 +529,9 @@ def head_decay_segments(tokens: int, sequences: int, dim: int, vdim: int) -> int
 
 
 @functools.lru_cache(maxsize=4096)
-def head_decay_tc_work(tokens: int, sequences: int, dim: int, vdim: int, tiles: int) -> int:
-    """Floats of scratch a head for the tcgen05 kernels of that attention, with segments of ``tiles`` times 128 tokens; 0: they do not
-    take such heads."""
-    return library().tb_head_decay_tc_work(tokens, sequences, dim, vdim, tiles)
+def head_decay_tc_work(tokens: int, sequences: int, dim: int, vdim: int) -> int:
+    """Floats of scratch a head for the tcgen05 kernels of that attention; 0: they do not take such heads."""
+    return library().tb_head_decay_tc_work(tokens, sequences, dim, vdim)
 
 
 def attention_window_mma_tile_tokens(nh: int, nkvh: int) -> int:

@@ -20,8 +20,6 @@ from .linear import matmul_nt
 MOST_DIM = 256                  # entries of a head, key or value
 MOST_ROWS = 2 ** 31 - 1         # tokens, sequences, slots: the kernels count them in 32 bits
 USE_TC = True                   # bfloat16 prompts: the tcgen05 kernels, for the heads that they take
-TILES = 2                       # tiles of 128 tokens in one of their segments: with 1 and 2, 2,048 tokens of 32 heads 60 and 51 us, 11,875 in 11
-                                # sequences 299 and 241 (twice the states' way through memory); 4 left the SMs with few long blocks
 WORK_BYTES = 256 << 20          # the most scratch for the segments' states: of more heads than it holds, portions are done in turn
 
 
@@ -128,10 +126,10 @@ def decay_attention(q, k, v, log_decay, state, seq_start, slots, out, *, scale=N
     if segments == 0:               # few tokens, small heads: one kernel does all
         lib.call("tb_head_decay_" + lib.suffix(q.dtype), *head, *rows, 0, 0, 1, nt, B, *more, stream=stream)
         return
-    per = lib.head_decay_tc_work(nt, B, dim, vdim, TILES) if q.dtype == torch.bfloat16 and USE_TC else 0
+    per = lib.head_decay_tc_work(nt, B, dim, vdim) if q.dtype == torch.bfloat16 and USE_TC else 0
     if per:
         heads, work = _work(per, H, q, scratch)
-        if lib.try_call("tb_head_decay_tc_bf16", *head, *rows, work.data_ptr(), TILES, heads, nt, B, *more, stream=stream):
+        if lib.try_call("tb_head_decay_tc_bf16", *head, *rows, work.data_ptr(), heads, nt, B, *more, stream=stream):
             return
     heads, work = _work(segments * (dim * vdim + 1), H, q, scratch)
     lib.call("tb_head_decay_" + lib.suffix(q.dtype), *head, *rows, work.data_ptr(), segments, heads, nt, B, *more, stream=stream)
