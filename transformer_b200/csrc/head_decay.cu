@@ -517,8 +517,11 @@ static void hd_rows_launch(const HeadDecayArgs& p, cudaStream_t s) {
     tb_allow_smem(allowed, (const void*)hd_rows_kernel<T, TILES>, ((size_t)HD_MAX_DIM + HD_SEG + 64) * HD_PAD * sizeof(float));
     TB_LAUNCH((hd_rows_kernel<T, TILES>), dim3(p.max_segs, p.heads), 256, smem, s, p);
 }
-// One kernel instead of three, and no scratch: heads of 64 x 64 in bfloat16, 33 tokens, 8 heads 12.6 us (the tcgen05 kernels 14.3), 33 tokens in 8
-// sequences of 32 heads 11.0 (25.0), 64 tokens of 8 heads 15.3 (14.1); the host's part of a call is 8 us less.
+// One kernel instead of three, and no scratch.  us of a call among others / of the kernels alone in a graph, this kernel and the three, heads
+// of 64 x 64: bfloat16 (the three on tcgen05), 8 heads, 8 tokens 15 / 9.7 and 24 / 13.5, 33 tokens 15 / 13.3 and 24 / 14.0, 64 tokens 17 / 16.7
+// and 24 / 13.9; 32 heads, 64 tokens in 8 sequences 15 / 11.4 and 26 / 24.6, in 32 sequences 35 / 34.9 and 64 / 62.9; float, 8 heads, 33 tokens
+// 15 / 11.1 and 22 / 19.5, 64 tokens 15 / 13.4 and 22 / 20.4, 32 heads in 32 sequences 33 / 33.1 and 70 / 69.1.  Where only the kernels
+// count, one bfloat16 sequence of more than some 35 tokens would have up to 4.5 us less with the three; prompts are calls, which are 7 us less with one.
 static bool hd_is_short(int nt, int dim, int vdim) { return nt <= HD_SEG && dim <= 64 && vdim <= 64; }
 
 // work: floats of scratch, `heads` heads of it (max_segs (dim vdim + 1) each); that many heads are done together.
