@@ -16,7 +16,7 @@
 // 2,039 tokens, 4 of 60, 4 us; 8 tokens 4 us.
 #include "common.cuh"
 
-#define RG_MAX_E 1024           // a power of two
+#define RG_MAX_E 1024
 #define RG_MAX_K 30
 #define RG_MAX_GROUPS 32
 #define RG_WARPS 8
@@ -126,30 +126,32 @@ __device__ __noinline__ int rg_choose64(const RouterGroupArgs& p, const float* r
                 if (i >= from && i < from + size) open &= ~(1u << i);
         }
     }
+    // larger value <=> larger key, NaN below -inf, 0 for what cannot be chosen (any more)
+    unsigned long long key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const unsigned long long b = (unsigned long long)__double_as_longlong(c[i] + 0.0);
+        key[i] = !(open >> i & 1u) ? 0ull : none >> i & 1u ? 1ull : b >> 63 ? ~b : b | 1ull << 63;
+    }
     int mine = 0;
     for (int j = 0; j < p.k; ++j) {
-        double best = lowest;
-        int at = 0x7fffffff;        // among equals the least; NaN stands behind -inf by a number above all experts'
+        unsigned long long best = key[0];
+        int at = 0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = lane * PER + i + (none >> i & 1u ? RG_MAX_E : 0);
-            if ((open >> i & 1u) && (at == 0x7fffffff || c[i] > best || (c[i] == best && e < at))) {
-                best = c[i];
-                at = e;
-            }
+        for (int i = 1; i < PER; ++i) {
+            at = key[i] > best ? i : at;
+            best = key[i] > best ? key[i] : best;
         }
+        // the largest of the warp by halves; the lowest lane among equals has the lowest index
+        const unsigned hi = (unsigned)(best >> 32), lo = (unsigned)best;
+        const unsigned most_hi = __reduce_max_sync(0xffffffffu, hi);
+        const unsigned most_lo = __reduce_max_sync(0xffffffffu, hi == most_hi ? lo : 0u);
+        const int from = __ffs(__ballot_sync(0xffffffffu, hi == most_hi && lo == most_lo)) - 1;
+        const int e = __shfl_sync(0xffffffffu, lane * PER + at, from);
+        if (lane == from)
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double ov = __shfl_xor_sync(0xffffffffu, best, o);
-            const int oi = __shfl_xor_sync(0xffffffffu, at, o);
-            if (oi != 0x7fffffff && (at == 0x7fffffff || ov > best || (ov == best && oi < at))) {
-                best = ov;
-                at = oi;
-            }
-        }
-        at &= RG_MAX_E - 1;
-        if (at / PER == lane) open &= ~(1u << (at - lane * PER));
-        if (lane == j) mine = at;
+            for (int i = 0; i < PER; ++i) key[i] = i == at ? 0ull : key[i];
+        if (lane == j) mine = e;
     }
     return mine;
 }
