@@ -8,8 +8,8 @@
 //   hd_step_kernel     one token per sequence: a block = a sequence x a head, the state once through the registers
 //
 // Segments of 64 tokens: the scores of a segment are one tile in shared memory.  Float throughout.  Bound by latency with few segments (a block of
-// 256 threads an SM) and by multiply-adds with many: 2 sequences of 200 to 700 tokens, 8 heads of 96 x 80 in float, update 16, pass 6, rows
-// with gate 30 us (60 the call; with plain multiply-adds instead of two an instruction 63).
+// 256 threads an SM) and by multiply-adds with many: 2 sequences of 200 to 700 tokens, 8 heads of 96 x 80 in float, update 17, pass 6, rows
+// with gate 31 us (59 the call; with plain multiply-adds instead of two an instruction 3 more).
 #include "head_decay.cuh"
 #include "memory_common.cuh"
 
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(256) hd_short_kernel(const HeadDecayArgs p) {
 
 // ---- one token per sequence ---------------------------------------------------------------------------------------
 // The state goes through the registers once, S' = e^g S + k v^T and its q^T S' on the way: bound by memory.  16 rows of 256 threads in flight, read and
-// written past the caches that others use: 64 sequences of 32 heads of 128 x 128 44 us, 6.1 TB/s (512 threads 63 us, 1,024 67); one
+// written past the caches that others use: 64 sequences of 32 heads of 128 x 128 45 us, 6.0 TB/s (512 threads 63 us, 1,024 67); one
 // sequence 6 us.
 // V: columns a thread and access (four where rows and heads are whole 16-byte pieces); NT threads, U rows asked for together.
 template <typename T, int V, int NT, int U>

@@ -17,8 +17,8 @@
 //
 // Bound by latency: copies, scores, weights, products and gate of a tile follow one another, some 12,000 clocks of which two blocks an SM (tensor
 // memory has room for no third) cover a part.  2,048 tokens of 32 heads of 128 x 128, us: update 18, pass 10, rows with
-// gate 30 (the call 50, 1.8 TB/s of what it has to read and write); 11,875 tokens in 11 sequences 78, 40,
-// 133; 8,192 tokens of 16 heads 32, 13, 53.
+// gate 30 (the call 50, 1.8 TB/s of what it has to read and write); 11,875 tokens in 11 sequences 79, 40, 131 (238); 8,192 tokens of 16 heads
+// 33, 13, 53 (90).
 #include <algorithm>
 
 #include "head_decay.cuh"
@@ -27,8 +27,9 @@
 
 #define HT_TILE 128
 #define HT_HALF 64              // rows of a TMA box, and keys that the update takes together
-#define HT_TILES 2              // tiles of a segment: with 1 and 2, 2,048 tokens of 32 heads 60 and 51 us, 11,875 in 11 sequences 299 and 241 (twice
-                                // the states' way through memory); 4 left the SMs with few long blocks (61 and 268)
+#define HT_TILES 2              // tiles of a segment.  us in a graph with 1 and 2: 2,048 tokens of 32 heads 57 and 48, 11,875 in 11 sequences 293 and
+                                // 236, 8,192 of 16 106 and 88 (twice the states' way through memory), 6 narrow sequences 40 and 38; 4 left the
+                                // SMs with few long blocks
 #define HT_SEG (HT_TILES * HT_TILE)
 #define HT_WORKERS 256          // eight warps: two for each 32 lanes of tensor memory, half of the columns each
 #define HT_THREADS (64 + HT_WORKERS)
@@ -874,8 +875,9 @@ static void ht_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtens
     tb_allow_smem(allowed_u, (const void*)hd_update_tc_kernel<KB, VB>, smem_u);
     tb_allow_smem(allowed_r, (const void*)hd_rows_tc_kernel<KB, VB>, smem_r);
     if (p.nt) TB_LAUNCH((hd_update_tc_kernel<KB, VB>), dim3(p.max_segs, (p.heads + a.heads_u - 1) / a.heads_u), HT_THREADS, smem_u, s, mk, mv, a);
-    // one wave of blocks is bound by the latency of its loads, more by memory: us of the whole call with 8 and 4 at a time, 8,192 tokens of 16
-    // heads of 128 87 and 99, 2,048 of 32 49.9 and 51.1, 11,875 in 11 sequences of 32 237 and 226
+    // one wave of blocks is bound by the latency of its loads, more by memory: us of the whole call in a graph with 8 and 4 at a time, 8,192 tokens
+    // of 16 heads of 128 88 and 99, 2,048 of 32 47.1 and 47.5, 6 sequences of 100 to 1,500 of 16 of 64 x 128 37.1 and 36.3 (all of one
+    // wave: 8), 11,875 in 11 sequences of 32 heads 250 and 235 (4.8 waves: 4)
     const dim3 grid(p.B, p.heads, (p.dim / 8 * ((p.vdim + 15) / 16) + 7) / 8);
     if ((long long)grid.x * grid.y * grid.z <= 148 * 8) TB_LAUNCH((hd_pass_tc_kernel<8>), grid, 256, 0, s, a);
     else TB_LAUNCH((hd_pass_tc_kernel<4>), grid, 256, 0, s, a);
@@ -919,9 +921,10 @@ int tb_head_decay_tc_bf16(const void* q, const void* k, const void* v, const voi
     a.error = tc_error_ptr();
     if (!a.error) return tb_last_error();
     // Heads a block: the next one's copies run ahead, but longer blocks leave the SMs less evenly.  Up to four, where three rounds of blocks
-    // over their places (two an SM) remain.  us of a call, 1, 2 and 4 heads a block of the update (with 2 of the rows) / of the rows (with 1 of
-    // the update): 11,875 tokens in 11 sequences of 32 heads of 128 245, 242 and 257 / 253, 245 and 245; 8,192 of 16 90.4, 88.5 and
-    // 94.3 / 91.2, 90.4 and 89.7; 2,048 of 32 50.9, 54.3 and 66.9 / 51.1, 50.9 and 64.1
+    // over their places (two an SM) remain.  us of a call in a graph, 1, 2 and 4 heads a block of the update / of the rows, the other by the
+    // rule: 11,875 tokens in 11 sequences of 32 heads of 128 239, 235 and 252 / 245, 236 and 235 (6 / 12 rounds: 2 / 4); 8,192 of 16 88, 85 and
+    // 91 / 88, 87 and 87 (1.8 / 3.6: 1); 2,048 of 32 47, 50 and 63 / 47, 48 and 60 (1 / 1.9: 1); 6 sequences of 100 to 1,500 of 16 heads of
+    // 64 x 128 37, 42 and 49 / 37, 36 and 46 (1.3 / 2.6: 1)
     const long long places = 2 * 148;
     auto per_block = [&](long long blocks) { return (int)std::max(1LL, std::min({4LL, (long long)heads, blocks * heads / (3 * places)})); };
     a.heads_u = per_block(p.max_segs);

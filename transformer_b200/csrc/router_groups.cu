@@ -12,8 +12,8 @@
 // a choice is one redux over order-preserving keys, a ballot and a shuffle.  Without a bias c and x have the same order, and the
 // logits themselves are compared.  With one, or where sums of scores decide, values closer than what float rounding can turn round
 // are decided again in 64 bits (float: expf 2 ulp, two more roundings, the sum's): a row in some hundreds.
-// Bound by integer and select instructions, some 1,370 a token: 8,191 tokens, the 8 of 256 experts in 4 of 8 groups, 14.5 us (0.6 TB/s of logits);
-// 2,039 tokens, 4 of 60, 4 us; 8 tokens 4 us.
+// Bound by integer and select instructions, some 1,370 a token: 8,191 tokens, the 8 of 256 experts in 4 of 8 groups, 16 us by itself and 14
+// behind another (0.6 TB/s of logits), of which a few rows in 64 bits are the last 1 to 3; 2,039 tokens, 4 of 60, 4 and 3 us; 8 tokens likewise.
 #include "common.cuh"
 
 #define RG_MAX_E 1024
