@@ -95,6 +95,8 @@ def _checked(q, k, v, log_decay, state, slots, out, norm, gate, new_state, seq_s
         ldgate, p_gate, p_norm = _rows(gate, "gate", nt, H, vdim, dtype), gate.data_ptr(), norm.data_ptr()
         if norm.dtype is not torch.float32 or norm.numel() != H * vdim or not norm.is_contiguous():
             raise ValueError(f"norm: a contiguous float32 tensor of [{H}, {vdim}], got {norm.dtype} {tuple(norm.shape)}")
+        if nt == 0:                 # a tensor without rows has no address, and there is nothing to gate
+            p_gate = p_norm = 0
     lib.check_device(q, k, v, log_decay, state, slots, out, norm, gate, new_state, seq_start)
     return (q.data_ptr(), k.data_ptr(), v.data_ptr(), p_gate, ldq, ldk, ldv, ldgate, log_decay.data_ptr(),
             max(strides[0], H) if each else 0, p_norm, state.data_ptr(), new_state.data_ptr(), pitch, new_pitch, out.data_ptr(),
