@@ -93,6 +93,24 @@ def test_a_worth_of_infinity_less_infinity(scores):
         _hold(x, 4, scores, bias, groups=4, groups_use=2, group_top=2)
 
 
+def test_logits_order_experts_of_equal_scores_however_their_groups_were_decided():
+    """Without a bias experts are compared by their logits, also where 64 bits have no scores between (sigmoids of 1, softmaxes of 0): in rows
+    whose groups are far apart, need no decision, or are equal and decided in 64 bits."""
+    from transformer_b200.parts import choose_experts
+
+    def chosen(row, k, scores, use):
+        idx, w = torch.empty((1, k), dtype=torch.int32, device="cuda"), torch.empty((1, k), device="cuda")
+        choose_experts(torch.tensor([row]).cuda(), idx, w, scores=scores, groups=2, groups_use=use, group_top=2)
+        return idx[0].tolist()
+
+    assert chosen([40.0, 41.0, -9.0, -8.0], 2, "sigmoid", 1) == [1, 0]
+    assert chosen([40.0, 41.0, 50.0, 60.0], 2, "sigmoid", 1) == [1, 0]
+    assert chosen([40.0, 41.0, 50.0, 60.0], 4, "sigmoid", 2) == [3, 2, 1, 0]
+    assert chosen([3e38, INF, 50.0, 60.0], 2, "sigmoid", 1) == [1, 0]
+    assert chosen([1.0, -900.0, -800.0, -999.0, 1.0, -950.0, -INF, NAN], 4, "sigmoid", 1) == [0, 2, 1, 3]
+    assert chosen([1.0, -900.0, -800.0, -999.0, 1.0, -950.0, -980.0, -INF], 4, "softmax", 1) == [0, 2, 1, 3]
+
+
 def test_the_most_tokens():
     """2^31 - 1 rows of one expert (26 GB): as many blocks as that is."""
     from transformer_b200.parts import choose_experts

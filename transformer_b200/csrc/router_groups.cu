@@ -126,6 +126,16 @@ __device__ __noinline__ int rg_choose64(const RouterGroupArgs& p, const float* r
                 if (i >= from && i < from + size) open &= ~(1u << i);
         }
     }
+    // without a bias experts are compared by their logits, here as everywhere
+    if (!p.bias) {
+        none = 0u;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const float x = lane * PER + i < p.E ? row[lane * PER + i] : 0.f;
+            c[i] = x;
+            none |= x != x ? 1u << i : 0u;
+        }
+    }
     // larger value <=> larger key, NaN below -inf, 0 for what cannot be chosen (any more)
     unsigned long long key[PER];
 #pragma unroll

@@ -43,7 +43,8 @@ def choose_experts(logits, index, weights, *, scores="softmax", bias=None, group
     Equal c, and groups of equal worth, go to the lower index.  A logit of -inf masks an expert: its score is 0, in a row of
     nothing else too, and where the chosen scores are all 0 their weights are 0 also with ``renorm``.  NaN ranks below -inf,
     counts as -inf in a group's worth (as inf - inf does) and spreads to the weights that it enters.  A row's indices always
-    differ.  What is decided on sums of scores, or on scores and a bias, is what 64 bits decide."""
+    differ.  Without a bias experts are compared by their logits; what is decided on sums of scores, or on scores and a bias, is
+    what 64 bits decide."""
     nt, E = logits.shape
     row, entry = logits.stride()
     k = index.shape[-1]
