@@ -10,8 +10,9 @@ head h of H reads those of head h // (H / G).  With ``norm`` and ``gate`` the he
 Sums, norms and the states that are carried are float on both paths, and single tokens, float prompts and the bfloat16 prompts that run on
 the CUDA cores (steps of up to 64 tokens with heads of up to 64, keys of more than 128 entries, sizes that are no multiples of eight, rows that are
 not whole 16-byte pieces) round each output once.  The other bfloat16 prompts run on the tensor cores, which take bfloat16: there the weights of a
-segment's tokens, and the copies of the states at the segments' starts that outputs are made from, are rounded to it too, so that an
-output's error is up to 1.5 times that of its last rounding.  The states that are carried do not see these copies.
+segment's tokens, and the copies of the states at the segments' starts that outputs are made from, are rounded to it too: 2^-8 of
+each term at most, over terms of random signs outputs that are some 1.4 times as far off as their last rounding alone makes them.  The states that
+are carried do not see these copies.
 Kernels: csrc/head_decay.cu, csrc/head_decay_tc.cu.
 """
 from __future__ import annotations
@@ -122,7 +123,8 @@ def decay_attention(q, k, v, log_decay, state, seq_start, slots, out, *, scale=N
     overlap anything else that the call reads.  Rows of ``out``
     behind the last sequence, and states that no sequence names, are left alone, as is all of a sequence whose bounds or slot lie
     outside the tensors.  A sequence without tokens keeps its state.  What is no number in v stays in its channel, behind its
-    token, a decay that is none in its head, from its token on; a gate far below 0 closes its channel.  ``scratch(name, shape, dtype)``: where the workspace comes from (default: allocated by the call)."""
+    token, a decay that is none in its head, from its token on; a gate far below 0 closes its channel.
+    ``scratch(name, shape, dtype)``: where the workspace comes from (default: allocated by the call)."""
     B, nt = slots.shape[0], q.shape[0]
     if seq_start.dtype != torch.int32 or seq_start.shape != (B + 1,) or not seq_start.is_contiguous():
         raise ValueError(f"seq_start must be a contiguous int32 tensor of {B + 1} entries")
