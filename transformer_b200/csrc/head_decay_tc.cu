@@ -8,8 +8,10 @@
 //
 // The states stay in float: K' is written as three bfloat16s, the value and what its rounding left twice (over K and beside it), and all are
 // multiplied with V into the same accumulator, so U has float's error (with two of them 2^-18 of a term may be left out, which showed: the
-// states were more than 1e-6 of their norm off).  P and S_0 enter products whose results are rounded to bfloat16 anyway, and are rounded to
-// it themselves.
+// states were more than 1e-6 of their norm off).  P, and the copy of S_0 that outputs are made from, are rounded to bfloat16 once: the outputs,
+// which are rounded to it themselves, are 2.1e-3 to 2.3e-3 of their norm off 64 bits instead of 1.7e-3.  Each in two bfloat16s they are 1.7e-3 off,
+// and a call in a graph takes, with P alone, with S_0 alone and with both so: 2,048 tokens of 32 heads 50, 54 and 55 us for 48; 11,875 in 11
+// sequences 253, 267 and 284 for 237; 8,192 of 16 92, 107 and 109 for 89.
 // A factor e^{c_i - c_j} is one exponential for a row and 32 keys times one for a key and the end of its 32, both at most 1; inside
 // the 32 x 32 on the diagonal, where the first would grow, one exponential each.  P takes its place over the scores in tensor memory (the A
 // operand of the second product).  Copies by TMA (3-D maps [tokens, heads, entries]: entries behind a head's are zeros), products issued
